@@ -67,11 +67,19 @@ SIGNATURES = {
     "iw_gelu_table": [_P, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P],
     "iw_gelu_table_tiled": [_P, _I64, _P, _P],
     "iw_shift_exp_table": [_I32, _P, _P],
+    "iw_paged_plan": [_P, _P],
+    "iw_paged_kv_write": [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P],
+    "iw_tree_attention": [_P, _P],
+    "iw_token_logprobs": [_P, _P],
     "iw_linear8_noalloc": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P],
 }
 
 IW_GEMM_ACC32, IW_GEMM_INT8, IW_GEMM_LINEAR32, IW_GEMM_LINEAR32_RES = 0, 1, 2, 3
 NOALLOC_MAX_ROWS = 65536  # IW_NOALLOC_MAX_ROWS
+# iw_paged_plan status bits (IW_PLAN_*), request limit; iw_token_logprobs limit
+PLAN_POOL_EXHAUSTED, PLAN_TABLE_TOO_SHORT, PLAN_TOO_MANY_TOKENS, PLAN_BAD_LENGTH, PLAN_TREE_TOO_LARGE = 1, 2, 4, 8, 16
+PLAN_MAX_REQUESTS = 16384
+LOGPROBS_MAX_TOP = 32
 
 
 class GemmDesc(C.Structure):
@@ -116,6 +124,41 @@ class GreedyDesc(C.Structure):
         ("suppress_bits", _P), ("blank", _P), ("n_blank", _I64),
         ("eot", _I64), ("timestamp_begin", _I64), ("no_timestamps", _I64), ("max_initial_timestamp_index", _I64),
         ("state", _P), ("tokens", _P), ("ld_tok", _I64), ("step_dev", _P), ("next", _P),
+    ]
+
+
+class PagedPlanDesc(C.Structure):
+    """``iw_paged_plan_desc`` (include/iwhisper_b200.h)."""
+    _fields_ = [
+        ("context_lens", _P), ("new_lens", _P), ("B", _I64),
+        ("block_table", _P), ("table_ld", _I64), ("table_width", _I64),
+        ("free_pages", _P), ("n_free", _I64), ("free_head", _P), ("page_size", _I64), ("max_tokens", _I64),
+        ("parents", _P), ("max_new", _I64),
+        ("slots", _P), ("request", _P), ("position", _P), ("tree_mask", _P), ("starts", _P), ("free_head_out", _P),
+        ("status", _P),
+    ]
+
+
+class TreeAttnDesc(C.Structure):
+    """``iw_tree_attn_desc`` (include/iwhisper_b200.h)."""
+    _fields_ = [
+        ("q", _P), ("ldq", _I64), ("q_hs", _I64), ("y", _P), ("ldy", _I64),
+        ("k_cache", _P), ("v_cache", _P),
+        ("page_stride", _I64), ("head_stride", _I64), ("row_stride", _I64), ("n_pages", _I64), ("page_size", _I64),
+        ("block_table", _P), ("table_ld", _I64), ("table_width", _I64),
+        ("context_lens", _P), ("starts", _P), ("tree_mask", _P), ("mask_words", _I64),
+        ("B", _I64), ("N", _I64), ("H", _I64), ("Hkv", _I64), ("D", _I64),
+        ("qk_multiplier", _U8), ("qk_shift", _I8), ("frac_bits", _I32),
+        ("av_multiplier", _U8), ("av_shift", _I8), ("rsqrt_offset", _I32),
+    ]
+
+
+class TokenLogprobsDesc(C.Structure):
+    """``iw_token_logprobs_desc`` (include/iwhisper_b200.h)."""
+    _fields_ = [
+        ("logits", _P), ("ld", _I64), ("dtype", C.c_int), ("N", _I64), ("V", _I64), ("scale", C.c_float),
+        ("suppress_bits", _P), ("targets", _P), ("C", _I64), ("top", _I64),
+        ("logprobs", _P), ("entropy", _P), ("top_ids", _P), ("top_logprobs", _P),
     ]
 
 

@@ -14,6 +14,7 @@
 #include "gemm_i8.cuh"
 #include "iw_common.cuh"
 #include "kernels.cuh"
+#include "paged.cuh"
 
 namespace {
 
@@ -713,6 +714,122 @@ int iw_log_mel_int8(const float *audio, int64_t B, int64_t n_samples, int64_t ld
     return cuda_check(iw::log_mel_int8(audio, (int)B, (int)n_samples, lda, filters, (int)n_mels, input_alpha,
                                        (float *)work.p, (int32_t *)wmax.p, out, st),
                       "iw_log_mel_int8");
+}
+
+// log2 of a page size, -1 when it is no power of two in [1, 2^20]
+static int page_log2(int64_t page_size) {
+    for (int l = 0; l <= 20; ++l)
+        if (page_size == (int64_t)1 << l) return l;
+    return -1;
+}
+
+static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int iw_paged_plan(const iw_paged_plan_desc *d, void *stream) {
+    if (!d) return fail(IW_EINVAL, "iw_paged_plan: null descriptor");
+    if (d->B < 1 || d->B > IW_PLAN_MAX_REQUESTS)
+        return fail(IW_EINVAL, "iw_paged_plan: the request count must be in [1, %d]", IW_PLAN_MAX_REQUESTS);
+    if (d->max_tokens < 0 || d->max_tokens >= INT32_MAX || d->n_free < 0 || d->n_free >= INT32_MAX || d->table_width < 0 ||
+        d->table_width > INT32_MAX || d->table_ld < d->table_width || d->table_width * 4 > INT64_MAX / d->B)
+        return fail(IW_EINVAL, "iw_paged_plan: invalid shape");
+    const int pl = page_log2(d->page_size);
+    if (pl < 0) return fail(IW_EINVAL, "iw_paged_plan: page_size must be a power of two, at most 2^20");
+    if (d->parents && (d->max_new < 1 || d->max_new > IW_PLAN_MAX_REQUESTS))
+        return fail(IW_EINVAL, "iw_paged_plan: max_new must be in [1, %d] with parents", IW_PLAN_MAX_REQUESTS);
+    if (!d->context_lens || !d->new_lens || !d->free_head || !d->starts || !d->free_head_out || !d->status ||
+        (d->table_width && !d->block_table) || (d->n_free && !d->free_pages) ||
+        (d->max_tokens && (!d->slots || !d->request || !d->position || (d->parents && !d->tree_mask))))
+        return fail(IW_EINVAL, "iw_paged_plan: null array");
+    if (d->free_head_out == d->free_head) return fail(IW_EINVAL, "iw_paged_plan: free_head_out must not be free_head");
+    iw::PlanArgs a;
+    a.ctx = d->context_lens; a.fresh = d->new_lens; a.B = (int)d->B;
+    a.table = d->block_table; a.table_ld = d->table_ld; a.width = (int)d->table_width;
+    a.free_pages = d->free_pages; a.n_free = d->n_free; a.free_head = d->free_head;
+    a.page_log2 = pl; a.max_tokens = d->max_tokens;
+    a.parents = d->parents; a.max_new = d->max_new; a.words = d->parents ? (int)((d->max_new + 31) / 32) : 0;
+    a.slots = d->slots; a.request = d->request; a.position = d->position; a.mask = d->tree_mask; a.starts = d->starts;
+    a.free_head_out = d->free_head_out; a.status = d->status;
+    return cuda_check(iw::paged_plan(a, S(stream)), "iw_paged_plan");
+}
+
+int iw_paged_kv_write(const int8_t *k, int64_t ldk, int64_t k_hs, const int8_t *v, int64_t ldv, int64_t v_hs,
+                      const int64_t *slots, int8_t *k_cache, int8_t *v_cache, int64_t page_stride,
+                      int64_t head_stride, int64_t row_stride, int64_t n_pages, int64_t page_size, int64_t N,
+                      int64_t H, int64_t D, void *stream) {
+    if (N < 0 || N > INT32_MAX || H < 1 || H > 65535 || D < 16 || D > 65536 || n_pages < 0 || n_pages > INT32_MAX)
+        return fail(IW_EINVAL, "iw_paged_kv_write: invalid shape");
+    const int pl = page_log2(page_size);
+    if (pl < 0) return fail(IW_EINVAL, "iw_paged_kv_write: page_size must be a power of two, at most 2^20");
+    if (N == 0 || n_pages == 0) return IW_OK;
+    if (!k || !v || !slots || !k_cache || !v_cache) return fail(IW_EINVAL, "iw_paged_kv_write: null array");
+    if (((D | ldk | k_hs | ldv | v_hs | page_stride | head_stride | row_stride) & 15) || !aligned16(k) || !aligned16(v) ||
+        !aligned16(k_cache) || !aligned16(v_cache))
+        return fail(IW_EINVAL, "iw_paged_kv_write: rows must be 16-byte aligned");
+    iw::KvWriteArgs a;
+    a.k = k; a.v = v; a.ldk = ldk; a.k_hs = k_hs; a.ldv = ldv; a.v_hs = v_hs; a.slots = slots;
+    a.k_cache = k_cache; a.v_cache = v_cache;
+    a.page_stride = page_stride; a.head_stride = head_stride; a.row_stride = row_stride;
+    a.n_slots = n_pages << pl; a.page_log2 = pl; a.H = (int)H; a.D = (int)D; a.N = N;
+    return cuda_check(iw::paged_kv_write(a, S(stream)), "iw_paged_kv_write");
+}
+
+int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
+    if (!d) return fail(IW_EINVAL, "iw_tree_attention: null descriptor");
+    if (d->B < 0 || d->B > 65535 || d->N < 0 || d->N > INT32_MAX || d->H < 1 || d->H > 4096 || d->Hkv < 1 || d->n_pages < 0 ||
+        d->n_pages > INT32_MAX || d->table_width < 0 || d->table_ld < d->table_width || d->mask_words < 0 ||
+        d->mask_words > IW_PLAN_MAX_REQUESTS)
+        return fail(IW_EINVAL, "iw_tree_attention: invalid shape");
+    if (d->H % d->Hkv) return fail(IW_EINVAL, "iw_tree_attention: the head count must be a multiple of the key head count");
+    if (d->D != 64 && d->D != 128) return fail(IW_EINVAL, "iw_tree_attention: head dimension must be 64 or 128");
+    const int pl = page_log2(d->page_size);
+    if (pl < 0) return fail(IW_EINVAL, "iw_tree_attention: page_size must be a power of two, at most 2^20");
+    // 255 * keys, the largest sum of probabilities, stays below 2^31
+    if (d->table_width > ((int64_t)1 << 23) >> pl)
+        return fail(IW_EINVAL, "iw_tree_attention: at most 2^23 keys per request");
+    if (!fused_frac_bits_ok(d->frac_bits)) return fail(IW_EINVAL, "frac_bits must be in [1, 30]");
+    if (!(d->rsqrt_offset >= 0 && d->rsqrt_offset <= 29)) return fail(IW_EINVAL, "rsqrt_offset must be in [0,29]");
+    if (d->N == 0) return IW_OK;
+    if (!d->q || !d->y || !d->starts || (d->B && !d->context_lens) ||
+        (d->B && d->table_width && !d->block_table) || (d->n_pages && (!d->k_cache || !d->v_cache)) ||
+        (d->tree_mask && !d->mask_words))
+        return fail(IW_EINVAL, "iw_tree_attention: null array");
+    if (((d->ldq | d->q_hs | d->ldy | d->page_stride | d->head_stride | d->row_stride) & 15) || !aligned16(d->q) ||
+        !aligned16(d->y) || !aligned16(d->k_cache) || !aligned16(d->v_cache))
+        return fail(IW_EINVAL, "iw_tree_attention: rows must be 16-byte aligned");
+    iw::TreeAttnArgs a;
+    a.q = d->q; a.ldq = d->ldq; a.q_hs = d->q_hs; a.y = d->y; a.ldy = d->ldy;
+    a.k = d->k_cache; a.v = d->v_cache;
+    a.page_stride = d->page_stride; a.head_stride = d->head_stride; a.row_stride = d->row_stride;
+    a.n_pages = d->n_pages; a.page_log2 = pl;
+    a.table = d->block_table; a.table_ld = d->table_ld; a.width = (int)d->table_width;
+    a.ctx = d->context_lens; a.starts = d->starts; a.mask = d->tree_mask;
+    a.words = d->tree_mask ? (int)d->mask_words : 0;
+    a.B = (int)d->B; a.H = (int)d->H; a.Hkv = (int)d->Hkv; a.D = (int)d->D; a.N = d->N;
+    a.qk_mult = d->qk_multiplier; a.qk_shift = (uint32_t)(d->qk_shift > 0 ? d->qk_shift : 0);
+    a.frac_bits = d->frac_bits; a.av_mult = d->av_multiplier;
+    a.av_shift = (uint32_t)iw::clampi(d->av_shift, 0, 32); a.rsqrt_offset = (uint32_t)d->rsqrt_offset;
+    return cuda_check(iw::tree_attention(a, S(stream)), "iw_tree_attention");
+}
+
+int iw_token_logprobs(const iw_token_logprobs_desc *d, void *stream) {
+    if (!d) return fail(IW_EINVAL, "iw_token_logprobs: null descriptor");
+    if (d->N < 0 || d->N > INT32_MAX || d->V < 1 || d->V > INT32_MAX || d->ld < d->V || d->C < 0)
+        return fail(IW_EINVAL, "iw_token_logprobs: invalid shape");
+    if (d->dtype < IW_LOGITS_INT8 || d->dtype > IW_LOGITS_FP32) return fail(IW_EINVAL, "iw_token_logprobs: bad dtype");
+    if (d->top < 0 || d->top > IW_LOGPROBS_MAX_TOP || d->top > d->V)
+        return fail(IW_EINVAL, "iw_token_logprobs: top must be in [0, min(V, %d)]", IW_LOGPROBS_MAX_TOP);
+    if (!(d->scale > 0.f) || d->scale > 3.0e38f) return fail(IW_EINVAL, "iw_token_logprobs: scale must be positive and finite");
+    if (d->N == 0) return IW_OK;
+    const int64_t size = d->dtype == IW_LOGITS_INT8 ? 1 : (d->dtype == IW_LOGITS_FP32 ? 4 : 2);
+    if (!d->logits || !d->entropy || (d->C && (!d->targets || !d->logprobs)) || (d->top && (!d->top_ids || !d->top_logprobs)))
+        return fail(IW_EINVAL, "iw_token_logprobs: null array");
+    if (reinterpret_cast<uintptr_t>(d->logits) % size)
+        return fail(IW_EINVAL, "iw_token_logprobs: logits must be aligned to their type");
+    iw::LogprobsArgs a;
+    a.x = d->logits; a.ld = d->ld; a.N = d->N; a.dtype = d->dtype; a.V = (int)d->V; a.scale = d->scale;
+    a.suppress = d->suppress_bits; a.targets = d->targets; a.C = d->C; a.top = (int)d->top;
+    a.lp = d->logprobs; a.entropy = d->entropy; a.top_ids = d->top_ids; a.top_lp = d->top_logprobs;
+    return cuda_check(iw::token_logprobs(a, S(stream)), "iw_token_logprobs");
 }
 
 int iw_add_i32(int32_t *p, int32_t v, void *stream) {

@@ -6,5 +6,8 @@
 #include "kernels.cu"
 #include "attn_tc.cu"
 #include "frontend.cu"
+#include "paged_plan.cu"
+#include "tree_attn.cu"
+#include "logprobs.cu"
 #include "capi.cu"
 #include "noalloc.cu"

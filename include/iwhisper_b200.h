@@ -430,6 +430,118 @@ int iw_log_mel_int8(const float *audio, int64_t B, int64_t n_samples, int64_t ld
 int iw_add_i32(int32_t *p, int32_t v, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Paged, tree-drafted decoding. These entry points have no counterpart in the
+ * reference, which decodes one token per utterance at one common position
+ * over dense caches: they serve ragged batches of requests, each with its own
+ * context in pages of a shared INT8 cache, and drafted token trees that are
+ * verified in one pass. Nothing here synchronises or allocates.
+ *
+ * A request b has context_lens[b] cached tokens and a number of new ones; the
+ * new tokens of all requests lie one after another, request b's at rows
+ * starts[b] .. starts[b+1]-1. Cache place p of a request is row p % page_size
+ * of page block_table[b][p / page_size]; new token t has place
+ * context_lens[b] + t. page_size is a power of two.
+ * ---------------------------------------------------------------------- */
+#define IW_PLAN_POOL_EXHAUSTED 1 /* fewer free pages than needed: some tokens have no slot  */
+#define IW_PLAN_TABLE_TOO_SHORT 2 /* a request needs more pages than block_table has columns */
+#define IW_PLAN_TOO_MANY_TOKENS 4 /* more new tokens than max_tokens: the rest is not planned */
+#define IW_PLAN_BAD_LENGTH 8     /* a length is negative or above 2^30: taken as 0          */
+#define IW_PLAN_TREE_TOO_LARGE 16 /* a request has more than max_new new tokens              */
+#define IW_PLAN_MAX_REQUESTS 16384
+
+typedef struct iw_paged_plan_desc {
+    const int32_t *context_lens, *new_lens; /* [B] */
+    int64_t B;
+    /* [B, table_width] at row stride table_ld. Columns below
+     * ceil(context/page_size) are read; the pages for the new tokens, taken in
+     * request order from free_pages[*free_head ...], are written behind them
+     * (-1 where the pool is exhausted). Other columns are left as they are. */
+    int32_t *block_table; int64_t table_ld, table_width;
+    const int32_t *free_pages; int64_t n_free;
+    const int32_t *free_head;     /* [1] first free page not yet taken               */
+    int64_t page_size, max_tokens;
+    /* optional: parents[i] is the index, within its request, of the token that
+     * row i follows; a value that is no earlier token of the request counts
+     * as -1, the end of the context. NULL: each request's tokens form a chain. */
+    const int32_t *parents;
+    int64_t max_new;              /* most new tokens of a request (tree_mask's width) */
+    /* outputs; rows from starts[B] up to max_tokens are padding            */
+    int64_t *slots;               /* [max_tokens] page*page_size + row, -1: none     */
+    int32_t *request;             /* [max_tokens] request of the row, -1: padding    */
+    int32_t *position;            /* [max_tokens] context + depth in the tree, 0: padding */
+    int32_t *tree_mask;           /* [max_tokens, ceil(max_new/32)] ancestor-or-self bits, 0: padding; only with parents */
+    int32_t *starts;              /* [B + 1]                                         */
+    int32_t *free_head_out;       /* [1]; not free_head itself (other blocks read it)   */
+    int32_t *status;              /* [1] IW_PLAN_* bits                              */
+} iw_paged_plan_desc;
+
+/* Block tables, slot map, positions and ancestor masks of one step, built on
+ * the device from the request lengths. */
+int iw_paged_plan(const iw_paged_plan_desc *d, void *stream);
+
+/* Rows (n, h) of k and v ([N, H, D] int8, element k[n*ldk + h*k_hs + d]) to
+ * row slots[n] % page_size of head h of page slots[n] / page_size of the
+ * caches; a page's element (h, r, d) is at page*page_stride + h*head_stride +
+ * r*row_stride + d, the same in both. Rows whose slot is negative or not
+ * below n_pages*page_size are skipped. D and all strides are multiples of 16
+ * bytes, pointers 16-byte aligned. Two rows with one slot leave either. */
+int iw_paged_kv_write(const int8_t *k, int64_t ldk, int64_t k_hs, const int8_t *v, int64_t ldv, int64_t v_hs,
+                      const int64_t *slots, int8_t *k_cache, int8_t *v_cache, int64_t page_stride,
+                      int64_t head_stride, int64_t row_stride, int64_t n_pages, int64_t page_size, int64_t N,
+                      int64_t H, int64_t D, void *stream);
+
+typedef struct iw_tree_attn_desc {
+    const int8_t *q; int64_t ldq, q_hs;  /* [N, H, D]: element q[n*ldq + h*q_hs + d] */
+    int8_t *y; int64_t ldy;              /* [N, H*D]                                 */
+    const int8_t *k_cache, *v_cache;     /* as in iw_paged_kv_write, Hkv heads       */
+    int64_t page_stride, head_stride, row_stride, n_pages, page_size;
+    const int32_t *block_table; int64_t table_ld, table_width;
+    const int32_t *context_lens;         /* [B]                                      */
+    const int32_t *starts;               /* [B + 1]                                  */
+    /* optional [N, mask_words]: new token i of a request sees its new token j
+     * when bit j%32 of word j/32 of row i is set (all of the context is always
+     * seen); NULL: each new token sees itself and those before it */
+    const int32_t *tree_mask; int64_t mask_words;
+    int64_t B, N, H, Hkv, D;             /* query head h reads key head h / (H/Hkv)   */
+    uint8_t qk_multiplier; int8_t qk_shift; int32_t frac_bits;
+    uint8_t av_multiplier; int8_t av_shift; int32_t rsqrt_offset;
+} iw_tree_attn_desc;
+
+/* The integer attention of iw_attention_ex for the new tokens of every
+ * request over its pages. D is 64 or 128. Keys whose page number is not in
+ * [0, n_pages) or whose place is past the block table are not seen; a row that
+ * sees no key gives 0, and rows from starts[B] up to N are set to 0. */
+int iw_tree_attention(const iw_tree_attn_desc *d, void *stream);
+
+#define IW_LOGITS_INT8 0
+#define IW_LOGITS_FP16 1
+#define IW_LOGITS_BF16 2
+#define IW_LOGITS_FP32 3
+#define IW_LOGPROBS_MAX_TOP 32
+
+typedef struct iw_token_logprobs_desc {
+    const void *logits; int64_t ld;      /* [N, V] at a row stride of ld elements     */
+    int dtype;                           /* IW_LOGITS_*                               */
+    int64_t N, V;
+    float scale;                         /* > 0: the logit of x is scale * x          */
+    const uint32_t *suppress_bits;       /* optional [ceil(V/32)]: bit id%32 of word id/32 removes id */
+    const int64_t *targets; int64_t C;   /* [N, C] given tokens                       */
+    int64_t top;                         /* alternatives per row, <= min(V, IW_LOGPROBS_MAX_TOP) */
+    float *logprobs;                     /* [N, C]                                    */
+    float *entropy;                      /* [N]                                       */
+    int64_t *top_ids; float *top_logprobs; /* [N, top]                                */
+} iw_token_logprobs_desc;
+
+/* Log probabilities of given tokens, the entropy (nats) and the most likely
+ * tokens of each row's softmax. A suppressed token and one whose logit is
+ * -inf have log probability -inf. Alternatives are ordered by logit, equal
+ * ones by id; where a row has fewer tokens than top, the rest have id -1 and
+ * -inf. A negative target gives 0 (padding), one of V or more NaN. A row that
+ * has no token left gives -inf, entropy 0 and no alternatives; one with a NaN or
+ * +inf that is not suppressed gives NaN and ids -1. */
+int iw_token_logprobs(const iw_token_logprobs_desc *d, void *stream);
+
+/* ------------------------------------------------------------------------
  * Allocation-free Linear8. This entry point has no counterpart in the
  * reference: it exists for callers that cannot allocate device memory while
  * they run -- work captured into a CUDA graph whose memory pool they do not
