@@ -5,6 +5,7 @@
 // wrap-around behaviour is spelled out with uint32 arithmetic.
 #pragma once
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <cstdlib>
