@@ -804,7 +804,8 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
     a.table = d->block_table; a.table_ld = d->table_ld; a.width = (int)d->table_width;
     a.ctx = d->context_lens; a.starts = d->starts; a.mask = d->tree_mask;
     a.words = d->tree_mask ? (int)d->mask_words : 0;
-    a.B = (int)d->B; a.H = (int)d->H; a.Hkv = (int)d->Hkv; a.D = (int)d->D; a.N = d->N;
+    a.B = (int)d->B; a.H = (int)d->H; a.Hkv = (int)d->Hkv; a.G = a.H / a.Hkv;
+    a.D = (int)d->D; a.N = d->N;
     a.qk_mult = d->qk_multiplier; a.qk_shift = (uint32_t)(d->qk_shift > 0 ? d->qk_shift : 0);
     a.frac_bits = d->frac_bits; a.av_mult = d->av_multiplier;
     a.av_shift = (uint32_t)iw::clampi(d->av_shift, 0, 32); a.rsqrt_offset = (uint32_t)d->rsqrt_offset;

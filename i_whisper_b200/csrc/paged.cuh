@@ -51,7 +51,7 @@ struct TreeAttnArgs {
     int width;
     const int32_t *ctx, *starts, *mask;
     int words;  // tree mask words per row (0: chains)
-    int B, H, Hkv, D;
+    int B, H, Hkv, G, D;  // G = H / Hkv
     int64_t N;
     int32_t qk_mult;
     uint32_t qk_shift;

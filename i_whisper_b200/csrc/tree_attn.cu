@@ -15,7 +15,7 @@ namespace tree {
 
 constexpr int kSlab = 32;  // keys per step of a warp
 
-// c += a (16 rows x 32, signed or unsigned bytes) * b (32 x 8 signed bytes).
+// c += a (16 rows x 32, signed bytes) * b (32 x 8 bytes, signed or unsigned).
 // Lane (g = lane/4, t = lane%4) holds a0/a1: rows g/g+8, k 4t..4t+3, a2/a3:
 // the same rows, k 16+4t..; b0/b1: column g, k 4t.. / 16+4t..; c0,c1/c2,c3:
 // rows g/g+8, columns 2t, 2t+1.
@@ -24,8 +24,8 @@ IW_DEV void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-IW_DEV void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+IW_DEV void mma_s8u8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -83,7 +83,7 @@ IW_DEV int32_t finish(const TreeAttnArgs &a, int32_t acc, int32_t inv) {
 // them, each its own heads.
 IW_DEV void zero_padding(const TreeAttnArgs &a, int kvh, int rank, int ranks) {
     const int64_t first = max(a.starts[a.B], 0);
-    const int G = a.H / a.Hkv, per = G * a.D / 16;
+    const int G = a.G, per = G * a.D / 16;
     for (int64_t i = (int64_t)rank * blockDim.x + threadIdx.x; i < (a.N - first) * per; i += (int64_t)ranks * blockDim.x)
         *reinterpret_cast<int4 *>(a.y + (first + i / per) * a.ldy + (int64_t)kvh * G * a.D + (i % per) * 16) =
             make_int4(0, 0, 0, 0);
@@ -93,22 +93,26 @@ IW_DEV void zero_padding(const TreeAttnArgs &a, int kvh, int rank, int ranks) {
 // Few rows per key head (single tokens, small trees): bound by reading K and V
 // once from HBM. A cluster of blocks serves one (request, key head) and
 // splits its keys; each warp streams slabs of 32 keys through a ring of its
-// own (cp.async, no block barrier), K first: 16 rows by 32 scores by
-// mma.sync, requantised scores kept in shared memory as 16 bits, so that K is
-// not read again once the maximum over all blocks is known (exchanged
-// through distributed shared memory); then V: probabilities, one thread per
-// (row, key), and P.V by mma.sync with V transposed by ldmatrix. mma.sync and
-// not tcgen05: with at most 16 rows the 128-row tile would be padding, and
-// the tensor pipe is far from the limit at HBM rate.
+// own (cp.async, no block barrier), K first: 32 scores by 8 rows by mma.sync
+// with the keys as the 16-row operand, the raw scores kept in shared memory so
+// that K is not read again once the maximum over all blocks is known
+// (exchanged through distributed shared memory; the requantisation is
+// monotone, so the maximum is taken of raw scores); then V: probabilities,
+// one thread per (row, key), and (P.V)^T by mma.sync with V transposed by
+// ldmatrix. mma.sync and not tcgen05: with at most 8 rows the 128-row tile
+// would be padding, and the tensor pipe is far from the limit at HBM rate.
 // ---------------------------------------------------------------------------
-constexpr int kFewWarps = 4;
-constexpr int kScoreLd = 80;  // bytes per row of a slab's scores: 32 x 16 bits, padded against bank conflicts
+constexpr int kFewRows = 8;
+constexpr int kScoreLd = 36;  // words per row of a slab's raw scores: 32, padded against bank conflicts
 
-template <int D>
+template <int D, int W>
 struct Few {
     static constexpr int kStages = D == 64 ? 4 : 3;
     static constexpr int kRing = kStages * kSlab * D;
-    static size_t smem(int score_cap) { return (size_t)kFewWarps * (kRing + score_cap) + 16 * D * 4 + 32 * 4; }
+    static constexpr int kOutLd = D + 4;
+    static size_t smem(int slots) {
+        return (size_t)W * (kRing + slots * kScoreLd * 4) + (kFewRows * kOutLd + 2 * kFewRows) * 4;
+    }
 };
 
 // 16-byte pieces of a slab's rows are swizzled so that the fragment loads are
@@ -119,34 +123,41 @@ IW_DEV int k_piece(int row, int c) { return D == 64 ? c : c ^ ((row & 1) << 2); 
 template <int D>
 IW_DEV int v_piece(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 3) : c ^ (row & 7); }
 
-template <int D>
-__global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a, int score_cap) {
+// D: head dimension, W: warps per block
+template <int D, int W>
+__global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kernel(TreeAttnArgs a, int slots) {
     namespace cg = cooperative_groups;
     pdl_wait();
     pdl_launch();
     extern __shared__ __align__(16) uint8_t smem[];
+    using F = Few<D, W>;
+    constexpr int S = F::kStages, OLD = F::kOutLd;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    constexpr int S = Few<D>::kStages;
-    uint8_t *ring = smem + warp * Few<D>::kRing;
-    uint8_t *score = smem + kFewWarps * Few<D>::kRing + warp * score_cap;
-    int32_t *s_o = reinterpret_cast<int32_t *>(smem + kFewWarps * (Few<D>::kRing + score_cap));  // [16][D]
-    int32_t *s_max = s_o + 16 * D, *s_sum = s_max + 16;
-    const int rank = blockIdx.x, ranks = gridDim.x, kvh = blockIdx.y, b = blockIdx.z;
-    const int G = a.H / a.Hkv;
+    uint8_t *ring = smem + warp * F::kRing;
+    int32_t *score = reinterpret_cast<int32_t *>(smem + W * F::kRing) + warp * slots * kScoreLd;
+    int32_t *s_o = reinterpret_cast<int32_t *>(smem + W * F::kRing) + W * slots * kScoreLd;
+    int32_t *s_sum = s_o + kFewRows * OLD, *s_max = s_sum + kFewRows;
+    const int rank = blockIdx.x, ranks = gridDim.x, kvh = blockIdx.y, b = blockIdx.z, G = a.G;
     if (b == a.B - 1) zero_padding(a, kvh, rank, ranks);
     const Request r = request(a, b);
     const int rows = r.fresh * G;
     if (rows == 0) return;
     const int64_t head_at = (int64_t)kvh * a.head_stride;
     const int slabs = (r.keys + kSlab - 1) / kSlab;
-    const int first = (int)((int64_t)slabs * rank / ranks), last = (int)((int64_t)slabs * (rank + 1) / ranks);
-    const int mine = max(0, (last - first - warp + kFewWarps - 1) / kFewWarps);
-    auto slab_at = [&](int i) { return (first + warp + i * kFewWarps) * kSlab; };
+    const int lr = 31 - __clz(ranks);  // a power of two
+    const int first = (slabs * rank) >> lr, last = (slabs * (rank + 1)) >> lr;
+    const int mine = max(0, (last - first - warp + W - 1) / W);
+    auto slab_at = [&](int i) { return (first + warp + i * W) * kSlab; };
+    auto token = [&](int row) { return G == 1 ? row : row / G; };
+    auto block_sync = [] {
+        if (W > 1) __syncthreads();
+        else __syncwarp();
+    };
     const RrsK rk = rrs_k(a.qk_shift);
 
-    for (int row0 = 0; row0 < rows; row0 += 16) {
-        const int nr = min(16, rows - row0);
-        const bool keep = mine * nr * kScoreLd <= score_cap;
+    for (int row0 = 0; row0 < rows; row0 += kFewRows) {
+        const int nr = min(kFewRows, rows - row0);
+        const bool keep = mine * nr <= slots;
         // the stream of slabs: K0 .. Kn-1, then V0 .. Vn-1, or K0 V0 K1 V1 ... when
         // the scores could not be kept
         const int items = mine * (keep ? 2 : 3);
@@ -154,13 +165,13 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
             if (it < items) {
                 const bool v = keep ? it >= mine : (it >= mine && ((it - mine) & 1));
                 const int i = it < mine ? it : (keep ? it - mine : (it - mine) >> 1);
-                const int j0 = slab_at(i);
+                const int64_t row_at = key_row(a, r, head_at, slab_at(i) + lane);
                 const int8_t *src = v ? a.v : a.k;
                 uint8_t *dst = ring + (it % S) * (kSlab * D);
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) {
                     const int row = (e * 32 + lane) / (D / 16), c = lane % (D / 16);
-                    const int64_t at = key_row(a, r, head_at, j0 + row);
+                    const int64_t at = __shfl_sync(0xffffffffu, row_at, row);
                     uint8_t *to = dst + row * D + (v ? v_piece<D>(row, c) : k_piece<D>(row, c)) * 16;
                     if (at >= 0) cp_async16(to, src + at + 16 * c);
                     else *reinterpret_cast<int4 *>(to) = make_int4(0, 0, 0, 0);
@@ -168,64 +179,64 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
             }
             cp_async_commit();
         };
+#pragma unroll 1
         for (int i = 0; i < S; ++i) issue(i);
 
-        // queries: lane's 16 bytes of rows g and g+8 in each 64-byte half, so that
-        // bytes 8s.. and 8s+4.. of the piece are a0 and a2 of step s
-        int4 q0[D / 64], q1[D / 64];
+        // queries: lane's 16 bytes of row g in each 64-byte half, so that bytes
+        // 8s.. and 8s+4.. of a piece are the two registers of step s (the same
+        // order of channels as in the keys' pieces below)
+        int4 q[D / 64];
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
-            q0[c] = q1[c] = make_int4(0, 0, 0, 0);
-            const int ra = row0 + g, rb = ra + 8;
-            if (ra < rows)
-                q0[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + ra / G) * a.ldq +
-                                                        (int64_t)(kvh * G + ra % G) * a.q_hs + 64 * c + 16 * t);
-            if (rb < rows)
-                q1[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + rb / G) * a.ldq +
-                                                        (int64_t)(kvh * G + rb % G) * a.q_hs + 64 * c + 16 * t);
+            q[c] = make_int4(0, 0, 0, 0);
+            const int row = row0 + g;
+            if (g < nr)
+                q[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + token(row)) * a.ldq +
+                                                       (int64_t)(kvh * G + row - token(row) * G) * a.q_hs + 64 * c + 16 * t);
         }
-        for (int i = tid; i < 16 * D + 32; i += 32 * kFewWarps) s_o[i] = i >= 16 * D && i < 16 * D + 16 ? -32768 : 0;
-        __syncthreads();
+        if (W > 1)
+            for (int i = tid; i < kFewRows * OLD + 2 * kFewRows; i += 32 * W)
+                s_o[i] = i < kFewRows * OLD + kFewRows ? 0 : INT32_MIN;
+        int holes = 0;  // a key of this block without a page
+        if (first < last)
+            for (int p = ((first * kSlab) >> a.page_log2) + tid; p <= (min(last * kSlab, r.keys) - 1) >> a.page_log2;
+                 p += 32 * W)
+                holes |= (uint32_t)r.table[p] >= (uint32_t)a.n_pages;
+        holes = W > 1 ? __syncthreads_or(holes) : __any_sync(0xffffffffu, holes);
 
-        int32_t m0 = -32768, m1 = -32768, mr = -32768;  // rows g, g + 8 (own columns); row = lane (masked slabs)
-        // whether every row sees every key of the slab, and which keys have a page
-        auto plain_slab = [&](int j0, uint32_t &there) {
-            there = __ballot_sync(0xffffffffu, key_row(a, r, head_at, j0 + lane) >= 0);
-            return there == 0xffffffffu && j0 + kSlab <= r.ctx;
-        };
-        // scores of a K slab in the ring -> score slot, and the running maximum
-        auto scores = [&](const uint8_t *ks, int j0, uint8_t *to, bool want_max, bool store) {
-            uint32_t there;
-            const bool plain = plain_slab(j0, there);
+        // whether every row sees every key of the slab
+        auto plain_slab = [&](int j0) { return !holes && j0 + kSlab <= min(r.ctx, r.keys); };
+        auto on = [&](int k, int j) { return key_row(a, r, head_at, j) >= 0 && sees(a, r, token(row0 + k), j); };
+        int32_t m0 = INT32_MIN, m1 = INT32_MIN, mr = INT32_MIN;  // rows 2t, 2t+1 (own keys); row = lane (other slabs)
+        // raw scores of a K slab in the ring, kept at `to`, and the running maximum
+        auto scores = [&](const uint8_t *ks, int j0, int32_t *to, bool want_max, bool store) {
+            const bool plain = plain_slab(j0);
 #pragma unroll
-            for (int n8 = 0; n8 < 4; ++n8) {
+            for (int m16 = 0; m16 < 2; ++m16) {
                 int32_t c[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
-                    const int row = 8 * n8 + g;
-                    const int4 k = *reinterpret_cast<const int4 *>(ks + row * D + k_piece<D>(row, 4 * h + t) * 16);
-                    mma_s8(c, q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
-                    mma_s8(c, q0[h].z, q1[h].z, q0[h].w, q1[h].w, k.z, k.w);
+                    const int row = 16 * m16 + g;
+                    const int4 ka = *reinterpret_cast<const int4 *>(ks + row * D + k_piece<D>(row, 4 * h + t) * 16);
+                    const int4 kb = *reinterpret_cast<const int4 *>(ks + (row + 8) * D + k_piece<D>(row, 4 * h + t) * 16);
+                    mma_s8(c, ka.x, kb.x, ka.y, kb.y, q[h].x, q[h].y);
+                    mma_s8(c, ka.z, kb.z, ka.w, kb.w, q[h].z, q[h].w);
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) c[e] = clampi(rrs_apply(wmul(c[e], a.qk_mult), rk), -32768, 32767);
                 if (plain) {
-                    m0 = max(m0, max(c[0], c[1]));
-                    m1 = max(m1, max(c[2], c[3]));
+                    m0 = max(m0, max(c[0], c[2]));
+                    m1 = max(m1, max(c[1], c[3]));
                 }
                 if (store || !plain) {
-                    uint8_t *w = to + 16 * n8 + 4 * t;
-                    if (g < nr) *reinterpret_cast<uint32_t *>(w + g * kScoreLd) = __byte_perm(c[0], c[1], 0x5410);
-                    if (g + 8 < nr) *reinterpret_cast<uint32_t *>(w + (g + 8) * kScoreLd) = __byte_perm(c[2], c[3], 0x5410);
+                    int32_t *w = to + 2 * t * kScoreLd + 16 * m16 + g;
+                    if (2 * t < nr) w[0] = c[0], w[8] = c[2];
+                    if (2 * t + 1 < nr) w[kScoreLd] = c[1], w[kScoreLd + 8] = c[3];
                 }
             }
             __syncwarp();
             if (want_max && !plain) {
-                for (int i = 0; i < nr; ++i) {
-                    const bool on = ((there >> lane) & 1) && sees(a, r, (row0 + i) / G, j0 + lane);
-                    const int32_t x = *reinterpret_cast<const int16_t *>(to + i * kScoreLd + 2 * lane);
-                    const int32_t m = __reduce_max_sync(0xffffffffu, on ? x : -32768);
-                    if (lane == i) mr = max(mr, m);
+                for (int k = 0; k < nr; ++k) {
+                    const int32_t m = __reduce_max_sync(0xffffffffu, on(k, j0 + lane) ? to[k * kScoreLd + lane] : INT32_MIN);
+                    if (lane == k) mr = max(mr, m);
                 }
                 __syncwarp();
             }
@@ -238,31 +249,40 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
             issue(it + S);
         }
         // row maxima: over the lanes, the warps, the cluster
-        m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, 1));
-        m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, 1));
-        m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, 2));
-        m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, 2));
-        if (t == 0) atomicMax(&s_max[g], m0), atomicMax(&s_max[g + 8], m1);
-        if (lane < nr) atomicMax(&s_max[lane], mr);
-        int32_t xm = -32768;  // row = lane
-        if (ranks == 1) {
-            __syncthreads();
-            if (lane < 16) xm = s_max[lane];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+            m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        }
+        int32_t xm;  // row = lane
+        if (W == 1) {
+            const int32_t e0 = __shfl_sync(0xffffffffu, m0, (lane >> 1) & 3), e1 = __shfl_sync(0xffffffffu, m1, (lane >> 1) & 3);
+            xm = max(mr, (lane & 1) ? e1 : e0);
+            if (ranks > 1 && lane < kFewRows) s_max[lane] = xm;
         } else {
+            if (g == 0) atomicMax(&s_max[2 * t], m0), atomicMax(&s_max[2 * t + 1], m1);
+            if (lane < nr && mr != INT32_MIN) atomicMax(&s_max[lane], mr);
+            if (ranks == 1) {
+                __syncthreads();
+                xm = s_max[lane & (kFewRows - 1)];
+            }
+        }
+        if (ranks > 1) {
             cg::cluster_group cl = cg::this_cluster();
             cl.sync();
-            if (lane < 16)
-                for (int k = 0; k < ranks; ++k) xm = max(xm, cl.map_shared_rank(s_max, k)[lane]);
+            xm = INT32_MIN;
+            for (int k = 0; k < ranks; ++k) xm = max(xm, cl.map_shared_rank(s_max, k)[lane & (kFewRows - 1)]);
         }
-        xm = (int16_t)(xm + 1);
+        auto requant = [&](int32_t acc) { return clampi(rrs_apply(wmul(acc, a.qk_mult), rk), -32768, 32767); };
+        xm = (int16_t)((xm == INT32_MIN ? -32768 : requant(xm)) + 1);
 
-        int32_t o[D / 8][4];
+        int32_t o[D / 16][4];  // channels 16i + g (and + 8) of rows 2t, 2t+1
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0;
-        int32_t sum0 = 0, sum1 = 0;
+        for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0;
+        uint32_t sum = 0;  // row g, own keys
         for (int i = 0; i < mine; ++i) {
             const int j0 = slab_at(i);
-            uint8_t *sc = score + (keep ? i * nr * kScoreLd : 0);
+            int32_t *sc = score + (keep ? i * nr * kScoreLd : 0);
             if (!keep) {
                 cp_async_wait<S - 1>();
                 __syncwarp();
@@ -270,35 +290,26 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
                 issue(it + S);
                 ++it;
             }
-            // probabilities in place of the scores: the row's first 32 bytes
-            uint32_t there;
-            const bool plain = plain_slab(j0, there);
+            // probabilities in place of the scores: the first 32 bytes of the row
+            const bool plain = plain_slab(j0);
             for (int k = 0; k < nr; ++k) {
                 const int32_t rm = __shfl_sync(0xffffffffu, xm, k);
-                const int32_t x = *reinterpret_cast<const int16_t *>(sc + k * kScoreLd + 2 * lane);
-                int32_t p = shift_exp_one(x, rm, a.frac_bits);
-                if (!plain && !(((there >> lane) & 1) && sees(a, r, (row0 + k) / G, j0 + lane))) p = 0;
+                int32_t p = shift_exp_one(requant(sc[k * kScoreLd + lane]), rm, a.frac_bits);
+                if (!plain && !on(k, j0 + lane)) p = 0;
                 __syncwarp();
-                sc[k * kScoreLd + lane] = (uint8_t)p;
+                reinterpret_cast<uint8_t *>(sc + k * kScoreLd)[lane] = (uint8_t)p;
             }
             cp_async_wait<S - 1>();
             __syncwarp();
             const uint8_t *vs = ring + (it % S) * (kSlab * D);
-            const uint8_t *pr = sc + g * kScoreLd + 4 * t;
-            uint32_t a0 = 0, a1 = 0, a2 = 0, a3 = 0;
-            if (g < nr) a0 = *reinterpret_cast<const uint32_t *>(pr), a2 = *reinterpret_cast<const uint32_t *>(pr + 16);
-            if (g + 8 < nr) {
-                a1 = *reinterpret_cast<const uint32_t *>(pr + 8 * kScoreLd);
-                a3 = *reinterpret_cast<const uint32_t *>(pr + 8 * kScoreLd + 16);
-            }
-            sum0 = (int32_t)__dp4a(a0, 0x01010101u, __dp4a(a2, 0x01010101u, (uint32_t)sum0));
-            sum1 = (int32_t)__dp4a(a1, 0x01010101u, __dp4a(a3, 0x01010101u, (uint32_t)sum1));
+            uint32_t p0 = 0, p1 = 0;
+            if (g < nr) p0 = sc[g * kScoreLd + t], p1 = sc[g * kScoreLd + 4 + t];
+            sum = __dp4a(p0, 0x01010101u, __dp4a(p1, 0x01010101u, sum));
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[4];
                 ldsm_trans_b8(v, vs + lane * D + v_piece<D>(lane, c) * 16);
-                mma_u8s8(o[2 * c], a0, a1, a2, a3, v[0], v[2]);
-                mma_u8s8(o[2 * c + 1], a0, a1, a2, a3, v[1], v[3]);
+                mma_s8u8(o[c], v[0], v[1], v[2], v[3], p0, p1);
             }
             __syncwarp();
             issue(it + S);
@@ -306,35 +317,36 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
         }
         cp_async_wait<0>();
         // sums over the warps, then over the cluster
-        sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
-        sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
-        sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
-        sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
-        if (mine) {
-            if (t == 0 && g < nr) atomicAdd(&s_sum[g], sum0);
-            if (t == 0 && g + 8 < nr) atomicAdd(&s_sum[g + 8], sum1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        auto give = [&](int32_t *d, int32_t v) {
+            if (W > 1) atomicAdd(d, v);
+            else *d = v;
+        };
+        if (W == 1 || mine) {
+            if (t == 0 && g < nr) give(&s_sum[g], (int32_t)sum);
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                int32_t *d = s_o + 8 * i + 2 * t;
-                if (g < nr) atomicAdd(d + g * D, o[i][0]), atomicAdd(d + g * D + 1, o[i][1]);
-                if (g + 8 < nr) atomicAdd(d + (g + 8) * D, o[i][2]), atomicAdd(d + (g + 8) * D + 1, o[i][3]);
+            for (int c = 0; c < D / 16; ++c) {
+                int32_t *d = s_o + 2 * t * OLD + 16 * c + g;
+                if (2 * t < nr) give(d, o[c][0]), give(d + 8, o[c][2]);
+                if (2 * t + 1 < nr) give(d + OLD, o[c][1]), give(d + OLD + 8, o[c][3]);
             }
         }
-        auto write = [&](auto total) {  // four channels per thread, rows dealt out over the cluster
-            for (int i = rank * 32 * kFewWarps + tid; i < nr * (D / 4); i += ranks * 32 * kFewWarps) {
+        auto write = [&](auto total) {  // four channels per thread, dealt out over the cluster
+            for (int i = rank * 32 * W + tid; i < nr * (D / 4); i += ranks * 32 * W) {
                 const int k = i / (D / 4), d = (i % (D / 4)) * 4, row = row0 + k;
                 const int32_t inv = fisr(total(s_sum, k), a.rsqrt_offset);
                 uint32_t w = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w |= (uint32_t)(finish(a, total(s_o, k * D + d + e), inv) & 255) << (8 * e);
-                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + row / G) * a.ldy +
-                                              (int64_t)(kvh * G + row % G) * D + d) = w;
+                for (int e = 0; e < 4; ++e) w |= (uint32_t)(finish(a, total(s_o, k * OLD + d + e), inv) & 255) << (8 * e);
+                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + token(row)) * a.ldy +
+                                              (int64_t)(kvh * G + row - token(row) * G) * D + d) = w;
             }
         };
         if (ranks == 1) {
-            __syncthreads();
+            block_sync();
             write([&](int32_t *p, int i) { return p[i]; });
-            __syncthreads();
+            block_sync();
         } else {
             cg::cluster_group cl = cg::this_cluster();
             cl.sync();
@@ -348,34 +360,55 @@ __global__ void __launch_bounds__(32 * kFewWarps) few_rows_kernel(TreeAttnArgs a
     }
 }
 
-template <int D>
-static cudaError_t few_rows(const TreeAttnArgs &a, cudaStream_t st) {
-    const int64_t keys = std::max<int64_t>(1, (int64_t)a.width << a.page_log2), pairs = (int64_t)a.B * a.Hkv;
-    // split the keys while the pairs alone leave SMs idle and a block keeps 256
-    // keys, or while a block would have more than 4096
-    int ranks = 1;
-    while (ranks < 8 && ((pairs * ranks < 3 * num_sms() && keys / ranks > 256) || keys / ranks > 4096)) ranks *= 2;
-    const int64_t per_warp = (keys / kSlab / ranks + kFewWarps) / kFewWarps;
-    const int64_t guess = std::min<int64_t>(16, std::max<int64_t>(1, (a.N + a.B - 1) / a.B * (a.H / a.Hkv)));
-    const int cap = (int)std::min<int64_t>(12 * 1024, std::max<int64_t>(16 * kScoreLd, per_warp * guess * kScoreLd));
-    const size_t smem = Few<D>::smem(cap);
-    static SmemLimit lim;
-    cudaError_t e = raise_smem_limit(few_rows_kernel<D>, smem, lim);
-    if (e != cudaSuccess) return e;
+// Kernel launch with the cluster size (blocks along x) and PDL attributes.
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                                  Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ranks, a.Hkv, a.B);
-    cfg.blockDim = dim3(32 * kFewWarps);
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled() ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = ranks;
+    attr[1].val.clusterDim.x = grid.x;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, few_rows_kernel<D>, a, cap);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int D, int W>
+static cudaError_t few_rows_launch(const TreeAttnArgs &a, int ranks, int slots, cudaStream_t st) {
+    const size_t smem = Few<D, W>::smem(slots);
+    static SmemLimit lim;
+    cudaError_t e = raise_smem_limit(few_rows_kernel<D, W>, smem, lim);
+    if (e != cudaSuccess) return e;
+    return launch_cluster(few_rows_kernel<D, W>, dim3(ranks, a.Hkv, a.B), dim3(32 * W), smem, st, a, slots);
+}
+
+template <int D>
+static cudaError_t few_rows(const TreeAttnArgs &a, cudaStream_t st) {
+    const int64_t keys = std::max<int64_t>(1, (int64_t)a.width << a.page_log2), pairs = (int64_t)a.B * a.Hkv;
+    // One warp per (request, key head) needs no barrier and shares no sums; more
+    // warps, then more blocks, while the SMs have fewer than 16 warps each and a
+    // warp keeps 64 keys, or while a warp would have more than 1024
+    int W = 1, ranks = 1;
+    while (W * ranks < 32) {
+        const int64_t share = keys / (W * ranks);
+        if (!((pairs * W * ranks < 16 * (int64_t)num_sms() && share > 64) || share > 1024)) break;
+        if (W < 4) W *= 2;
+        else ranks *= 2;
+    }
+    // room for the scores of every slab, at the mean row count of the batch
+    const int64_t per_warp = (keys / kSlab / ranks + W) / W;
+    const int64_t guess = std::min<int64_t>(kFewRows, std::max<int64_t>(1, (a.N + a.B - 1) / a.B * a.G));
+    const int slots = (int)std::min<int64_t>(64, std::max<int64_t>(kFewRows, per_warp * guess));
+    if (W == 1) return few_rows_launch<D, 1>(a, ranks, slots, st);
+    if (W == 2) return few_rows_launch<D, 2>(a, ranks, slots, st);
+    return few_rows_launch<D, 4>(a, ranks, slots, st);
 }
 
 }  // namespace tree
