@@ -796,11 +796,14 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
     if (((d->ldq | d->q_hs | d->ldy | d->page_stride | d->head_stride | d->row_stride) & 15) || !aligned16(d->q) ||
         !aligned16(d->y) || !aligned16(d->k_cache) || !aligned16(d->v_cache))
         return fail(IW_EINVAL, "iw_tree_attention: rows must be 16-byte aligned");
+    if (d->page_stride < 0 || d->row_stride < 0 || d->page_stride > INT32_MAX || d->row_stride > INT32_MAX)
+        return fail(IW_EINVAL, "iw_tree_attention: page and row strides must be below 2^31 bytes");
     iw::TreeAttnArgs a;
     a.q = d->q; a.ldq = d->ldq; a.q_hs = d->q_hs; a.y = d->y; a.ldy = d->ldy;
     a.k = d->k_cache; a.v = d->v_cache;
-    a.page_stride = d->page_stride; a.head_stride = d->head_stride; a.row_stride = d->row_stride;
-    a.n_pages = d->n_pages; a.page_log2 = pl;
+    a.head_stride = d->head_stride;
+    a.page_stride = (uint32_t)d->page_stride; a.row_stride = (uint32_t)d->row_stride; a.n_pages = (uint32_t)d->n_pages;
+    a.page_log2 = pl;
     a.table = d->block_table; a.table_ld = d->table_ld; a.width = (int)d->table_width;
     a.ctx = d->context_lens; a.starts = d->starts; a.mask = d->tree_mask;
     a.words = d->tree_mask ? (int)d->mask_words : 0;

@@ -44,7 +44,8 @@ struct TreeAttnArgs {
     int8_t *y;
     int64_t ldy;
     const int8_t *k, *v;
-    int64_t page_stride, head_stride, row_stride, n_pages;
+    int64_t head_stride;
+    uint32_t page_stride, row_stride, n_pages;
     int page_log2;
     const int32_t *table;
     int64_t table_ld;

@@ -56,12 +56,31 @@ IW_DEV Request request(const TreeAttnArgs &a, int b) {
     return r;
 }
 
-// Byte offset of key j's row of one head in the caches, -1 when it has no page.
-IW_DEV int64_t key_row(const TreeAttnArgs &a, const Request &r, int64_t head_at, int j) {
-    if (j >= r.keys) return -1;
-    const int32_t page = r.table[j >> a.page_log2];
-    if ((uint32_t)page >= (uint32_t)a.n_pages) return -1;
-    return page * a.page_stride + head_at + (j & ((1 << a.page_log2) - 1)) * a.row_stride;
+// Byte offset of row j of a page within the caches' head.
+IW_DEV uint64_t row_at(const TreeAttnArgs &a, int32_t page, int j) {
+    return (uint64_t)(uint32_t)page * a.page_stride + (uint64_t)((uint32_t)j & ((1u << a.page_log2) - 1)) * a.row_stride;
+}
+IW_DEV bool has_page(const TreeAttnArgs &a, const Request &r, int j) {
+    return j < r.keys && (uint32_t)r.table[j >> a.page_log2] < a.n_pages;
+}
+
+// (x - M - 1) -> the probability, x <= M the requantised score: shift_exp_one
+// by fewer steps where the exponent's fraction has 7 to 14 bits. With
+// d = x - M - 1 in [-65536, -1]: the 16-bit steps of the definition wrap where
+// d < -22795, which then gives 0 (a positive exponent), and d = -65536 wraps to 0,
+// the largest probability.
+struct ExpK {
+    int32_t fb, one, mask, sh;
+    bool quick;
+};
+IW_DEV ExpK exp_k(int32_t fb) { return {fb, 1 << (fb & 15), (1 << (fb & 15)) - 1, fb - 7, fb >= 7 && fb <= 14}; }
+IW_DEV int32_t quick_exp(int32_t d, const ExpK &k) {
+    const int32_t f = d + (d >> 1) - (d >> 4);
+    const uint32_t num = (uint32_t)(((f & k.mask) >> 1) + k.one);
+    int32_t p;
+    asm("shr.u32 %0, %1, %2;" : "=r"(p) : "r"(num), "r"(k.sh - (f >> k.fb)));  // 0 for shifts above 31
+    if (d < -22795) p = d == -65536 ? 128 : 0;
+    return p;
 }
 
 // Whether new token t of the request sees key j, which has a page.
@@ -91,23 +110,24 @@ IW_DEV void zero_padding(const TreeAttnArgs &a, int kvh, int rank, int ranks) {
 
 // ---------------------------------------------------------------------------
 // Few rows per key head (single tokens, small trees): bound by reading K and V
-// once from HBM. A cluster of blocks serves one (request, key head) and
-// splits its keys; each warp streams slabs of 32 keys through a ring of its
-// own (cp.async, no block barrier), K first: 32 scores by 8 rows by mma.sync
-// with the keys as the 16-row operand, the raw scores kept in shared memory so
-// that K is not read again once the maximum over all blocks is known
-// (exchanged through distributed shared memory; the requantisation is
-// monotone, so the maximum is taken of raw scores); then V: probabilities,
-// one thread per (row, key), and (P.V)^T by mma.sync with V transposed by
-// ldmatrix. mma.sync and not tcgen05: with at most 8 rows the 128-row tile
-// would be padding, and the tensor pipe is far from the limit at HBM rate.
+// once from HBM. Blocks of one to four warps, or a cluster of them, serve one
+// (request, key head) and split its keys; each warp streams slabs of 32 keys
+// through a ring of its own (cp.async, no block barrier), K first: 32 scores by
+// 8 rows by mma.sync with the keys as the 16-row operand, the raw scores kept in
+// shared memory so that K is not read again once the maximum over all
+// blocks is known (exchanged through distributed shared memory; the
+// requantisation is monotone, so the maximum is taken of raw scores); then V:
+// probabilities, one thread per (row, key), and (P.V)^T by mma.sync with V
+// transposed by ldmatrix. mma.sync and not tcgen05: with at most 8 rows the
+// 128-row tile would be padding, and the tensor pipe is far from its limit at
+// HBM rate; what counts is the instructions per slab.
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 8;
 constexpr int kScoreLd = 36;  // words per row of a slab's raw scores: 32, padded against bank conflicts
 
 template <int D, int W>
 struct Few {
-    static constexpr int kStages = D == 64 ? 4 : 3;
+    static constexpr int kStages = 4;
     static constexpr int kRing = kStages * kSlab * D;
     static constexpr int kOutLd = D + 4;
     static size_t smem(int slots) {
@@ -125,7 +145,7 @@ IW_DEV int v_piece(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 3) : c ^
 
 // D: head dimension, W: warps per block
 template <int D, int W>
-__global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kernel(TreeAttnArgs a, int slots) {
+__global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kernel(TreeAttnArgs a, int slots) {
     namespace cg = cooperative_groups;
     pdl_wait();
     pdl_launch();
@@ -142,38 +162,41 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kern
     const Request r = request(a, b);
     const int rows = r.fresh * G;
     if (rows == 0) return;
-    const int64_t head_at = (int64_t)kvh * a.head_stride;
+    const int8_t *kbase = a.k + kvh * a.head_stride, *vbase = a.v + kvh * a.head_stride;
     const int slabs = (r.keys + kSlab - 1) / kSlab;
     const int lr = 31 - __clz(ranks);  // a power of two
     const int first = (slabs * rank) >> lr, last = (slabs * (rank + 1)) >> lr;
     const int mine = max(0, (last - first - warp + W - 1) / W);
     auto slab_at = [&](int i) { return (first + warp + i * W) * kSlab; };
+    int holes = 0;  // a key of this block without a page
+    if (first < last)
+        for (int p = ((first * kSlab) >> a.page_log2) + lane; p <= (min(last * kSlab, r.keys) - 1) >> a.page_log2; p += 32)
+            holes |= (uint32_t)r.table[p] >= a.n_pages;
+    holes = __any_sync(0xffffffffu, holes);
     auto token = [&](int row) { return G == 1 ? row : row / G; };
     auto block_sync = [] {
         if (W > 1) __syncthreads();
         else __syncwarp();
     };
     const RrsK rk = rrs_k(a.qk_shift);
+    const ExpK ek = exp_k(a.frac_bits);
 
     for (int row0 = 0; row0 < rows; row0 += kFewRows) {
         const int nr = min(kFewRows, rows - row0);
-        const bool keep = mine * nr <= slots;
-        // the stream of slabs: K0 .. Kn-1, then V0 .. Vn-1, or K0 V0 K1 V1 ... when
-        // the scores could not be kept
-        const int items = mine * (keep ? 2 : 3);
-        auto issue = [&](int it) {
-            if (it < items) {
-                const bool v = keep ? it >= mine : (it >= mine && ((it - mine) & 1));
-                const int i = it < mine ? it : (keep ? it - mine : (it - mine) >> 1);
-                const int64_t row_at = key_row(a, r, head_at, slab_at(i) + lane);
-                const int8_t *src = v ? a.v : a.k;
-                uint8_t *dst = ring + (it % S) * (kSlab * D);
+        const bool keep = mine * nr <= slots;  // otherwise the second pass computes the scores again
+        auto issue = [&](int it) {             // the stream of slabs: K0 .. Kn-1, V0 .. Vn-1
+            if (it < 2 * mine) {
+                const bool v = it >= mine;
+                const int j0 = slab_at(v ? it - mine : it);
+                const int8_t *src = (v ? vbase : kbase) + 16 * (lane % (D / 16));
+                uint8_t *dst = ring + (it & (S - 1)) * (kSlab * D);
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) {
                     const int row = (e * 32 + lane) / (D / 16), c = lane % (D / 16);
-                    const int64_t at = __shfl_sync(0xffffffffu, row_at, row);
+                    const int j = min(j0 + row, r.keys - 1);  // rows past the end repeat the last: they are masked
+                    const int32_t page = r.table[j >> a.page_log2];
                     uint8_t *to = dst + row * D + (v ? v_piece<D>(row, c) : k_piece<D>(row, c)) * 16;
-                    if (at >= 0) cp_async16(to, src + at + 16 * c);
+                    if (!holes || (uint32_t)page < a.n_pages) cp_async16(to, src + row_at(a, page, j));
                     else *reinterpret_cast<int4 *>(to) = make_int4(0, 0, 0, 0);
                 }
             }
@@ -189,63 +212,68 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kern
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) {
             q[c] = make_int4(0, 0, 0, 0);
-            const int row = row0 + g;
+            const int row = row0 + g, n = token(row);
             if (g < nr)
-                q[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + token(row)) * a.ldq +
-                                                       (int64_t)(kvh * G + row - token(row) * G) * a.q_hs + 64 * c + 16 * t);
+                q[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + n) * a.ldq +
+                                                       (int64_t)(kvh * G + row - n * G) * a.q_hs + 64 * c + 16 * t);
         }
-        if (W > 1)
+        if (W > 1) {
             for (int i = tid; i < kFewRows * OLD + 2 * kFewRows; i += 32 * W)
                 s_o[i] = i < kFewRows * OLD + kFewRows ? 0 : INT32_MIN;
-        int holes = 0;  // a key of this block without a page
-        if (first < last)
-            for (int p = ((first * kSlab) >> a.page_log2) + tid; p <= (min(last * kSlab, r.keys) - 1) >> a.page_log2;
-                 p += 32 * W)
-                holes |= (uint32_t)r.table[p] >= (uint32_t)a.n_pages;
-        holes = W > 1 ? __syncthreads_or(holes) : __any_sync(0xffffffffu, holes);
+            __syncthreads();
+        }
 
         // whether every row sees every key of the slab
         auto plain_slab = [&](int j0) { return !holes && j0 + kSlab <= min(r.ctx, r.keys); };
-        auto on = [&](int k, int j) { return key_row(a, r, head_at, j) >= 0 && sees(a, r, token(row0 + k), j); };
+        auto on = [&](int k, int j) { return has_page(a, r, j) && sees(a, r, token(row0 + k), j); };
         int32_t m0 = INT32_MIN, m1 = INT32_MIN, mr = INT32_MIN;  // rows 2t, 2t+1 (own keys); row = lane (other slabs)
-        // raw scores of a K slab in the ring, kept at `to`, and the running maximum
-        auto scores = [&](const uint8_t *ks, int j0, int32_t *to, bool want_max, bool store) {
-            const bool plain = plain_slab(j0);
+        // raw scores of the keys 16m + g and 16m + 8 + g with all rows; load(row, h)
+        // gives the lane's piece of a key's half h
+        auto raw = [&](int32_t (&c)[2][4], auto load) {
 #pragma unroll
             for (int m16 = 0; m16 < 2; ++m16) {
-                int32_t c[4] = {0, 0, 0, 0};
+                c[m16][0] = c[m16][1] = c[m16][2] = c[m16][3] = 0;
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
-                    const int row = 16 * m16 + g;
-                    const int4 ka = *reinterpret_cast<const int4 *>(ks + row * D + k_piece<D>(row, 4 * h + t) * 16);
-                    const int4 kb = *reinterpret_cast<const int4 *>(ks + (row + 8) * D + k_piece<D>(row, 4 * h + t) * 16);
-                    mma_s8(c, ka.x, kb.x, ka.y, kb.y, q[h].x, q[h].y);
-                    mma_s8(c, ka.z, kb.z, ka.w, kb.w, q[h].z, q[h].w);
-                }
-                if (plain) {
-                    m0 = max(m0, max(c[0], c[2]));
-                    m1 = max(m1, max(c[1], c[3]));
-                }
-                if (store || !plain) {
-                    int32_t *w = to + 2 * t * kScoreLd + 16 * m16 + g;
-                    if (2 * t < nr) w[0] = c[0], w[8] = c[2];
-                    if (2 * t + 1 < nr) w[kScoreLd] = c[1], w[kScoreLd + 8] = c[3];
+                    const int4 ka = load(16 * m16 + g, h), kb = load(16 * m16 + 8 + g, h);
+                    mma_s8(c[m16], ka.x, kb.x, ka.y, kb.y, q[h].x, q[h].y);
+                    mma_s8(c[m16], ka.z, kb.z, ka.w, kb.w, q[h].z, q[h].w);
                 }
             }
+        };
+        auto store = [&](int32_t *to, const int32_t (&c)[2][4]) {
+            int32_t *w = to + 2 * t * kScoreLd + g;
+            if (2 * t < nr) w[0] = c[0][0], w[8] = c[0][2], w[16] = c[1][0], w[24] = c[1][2];
+            if (2 * t + 1 < nr) {
+                w += kScoreLd;
+                w[0] = c[0][1], w[8] = c[0][3], w[16] = c[1][1], w[24] = c[1][3];
+            }
+        };
+        int it = 0;
+#pragma unroll 1
+        for (; it < mine; ++it) {
+            const int j0 = slab_at(it);
+            cp_async_wait<S - 1>();
             __syncwarp();
-            if (want_max && !plain) {
+            const uint8_t *ks = ring + (it & (S - 1)) * (kSlab * D);
+            int32_t c[2][4];
+            raw(c, [&](int row, int h) {
+                return *reinterpret_cast<const int4 *>(ks + row * D + k_piece<D>(row, 4 * h + t) * 16);
+            });
+            const bool plain = plain_slab(j0);
+            int32_t *to = score + (keep ? it * nr * kScoreLd : 0);
+            if (plain) {
+                m0 = max(max(m0, max(c[0][0], c[0][2])), max(c[1][0], c[1][2]));
+                m1 = max(max(m1, max(c[0][1], c[0][3])), max(c[1][1], c[1][3]));
+            }
+            if (keep || !plain) store(to, c);
+            __syncwarp();
+            if (!plain)
                 for (int k = 0; k < nr; ++k) {
                     const int32_t m = __reduce_max_sync(0xffffffffu, on(k, j0 + lane) ? to[k * kScoreLd + lane] : INT32_MIN);
                     if (lane == k) mr = max(mr, m);
                 }
-                __syncwarp();
-            }
-        };
-        int it = 0;
-        for (int i = 0; i < mine; ++i, ++it) {
-            cp_async_wait<S - 1>();
             __syncwarp();
-            scores(ring + (it % S) * (kSlab * D), slab_at(i), score + (keep ? i * nr * kScoreLd : 0), true, keep);
             issue(it + S);
         }
         // row maxima: over the lanes, the warps, the cluster
@@ -274,46 +302,51 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kern
             for (int k = 0; k < ranks; ++k) xm = max(xm, cl.map_shared_rank(s_max, k)[lane & (kFewRows - 1)]);
         }
         auto requant = [&](int32_t acc) { return clampi(rrs_apply(wmul(acc, a.qk_mult), rk), -32768, 32767); };
-        xm = (int16_t)((xm == INT32_MIN ? -32768 : requant(xm)) + 1);
+        xm = (xm == INT32_MIN ? -32768 : requant(xm)) + 1;
 
         int32_t o[D / 16][4];  // channels 16i + g (and + 8) of rows 2t, 2t+1
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0;
         uint32_t sum = 0;  // row g, own keys
-        for (int i = 0; i < mine; ++i) {
-            const int j0 = slab_at(i);
+#pragma unroll 1
+        for (; it < 2 * mine; ++it) {
+            const int i = it - mine, j0 = slab_at(i);
             int32_t *sc = score + (keep ? i * nr * kScoreLd : 0);
             if (!keep) {
-                cp_async_wait<S - 1>();
+                int32_t c[2][4];
+                raw(c, [&](int row, int h) {
+                    const int j = min(j0 + row, r.keys - 1);
+                    const int32_t page = r.table[j >> a.page_log2];
+                    if (holes && (uint32_t)page >= a.n_pages) return make_int4(0, 0, 0, 0);
+                    return *reinterpret_cast<const int4 *>(kbase + row_at(a, page, j) + 64 * h + 16 * t);
+                });
+                store(sc, c);
                 __syncwarp();
-                scores(ring + (it % S) * (kSlab * D), j0, sc, false, true);
-                issue(it + S);
-                ++it;
             }
             // probabilities in place of the scores: the first 32 bytes of the row
             const bool plain = plain_slab(j0);
             for (int k = 0; k < nr; ++k) {
                 const int32_t rm = __shfl_sync(0xffffffffu, xm, k);
-                int32_t p = shift_exp_one(requant(sc[k * kScoreLd + lane]), rm, a.frac_bits);
+                const int32_t x = requant(sc[k * kScoreLd + lane]);
+                int32_t p = ek.quick ? quick_exp(x - rm, ek) : shift_exp_one(x, (int16_t)rm, a.frac_bits);
                 if (!plain && !on(k, j0 + lane)) p = 0;
                 __syncwarp();
                 reinterpret_cast<uint8_t *>(sc + k * kScoreLd)[lane] = (uint8_t)p;
             }
             cp_async_wait<S - 1>();
             __syncwarp();
-            const uint8_t *vs = ring + (it % S) * (kSlab * D);
+            const uint8_t *vs = ring + (it & (S - 1)) * (kSlab * D) + lane * D;
             uint32_t p0 = 0, p1 = 0;
             if (g < nr) p0 = sc[g * kScoreLd + t], p1 = sc[g * kScoreLd + 4 + t];
             sum = __dp4a(p0, 0x01010101u, __dp4a(p1, 0x01010101u, sum));
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[4];
-                ldsm_trans_b8(v, vs + lane * D + v_piece<D>(lane, c) * 16);
+                ldsm_trans_b8(v, vs + v_piece<D>(lane, c) * 16);
                 mma_s8u8(o[c], v[0], v[1], v[2], v[3], p0, p1);
             }
             __syncwarp();
             issue(it + S);
-            ++it;
         }
         cp_async_wait<0>();
         // sums over the warps, then over the cluster
@@ -325,22 +358,24 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 24 : 16) / W) few_rows_kern
         };
         if (W == 1 || mine) {
             if (t == 0 && g < nr) give(&s_sum[g], (int32_t)sum);
+            int32_t *d = s_o + 2 * t * OLD + g;
+            if (2 * t < nr) {
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {
-                int32_t *d = s_o + 2 * t * OLD + 16 * c + g;
-                if (2 * t < nr) give(d, o[c][0]), give(d + 8, o[c][2]);
-                if (2 * t + 1 < nr) give(d + OLD, o[c][1]), give(d + OLD + 8, o[c][3]);
+                for (int c = 0; c < D / 16; ++c) give(d + 16 * c, o[c][0]), give(d + 16 * c + 8, o[c][2]);
+            }
+            if (2 * t + 1 < nr) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) give(d + OLD + 16 * c, o[c][1]), give(d + OLD + 16 * c + 8, o[c][3]);
             }
         }
         auto write = [&](auto total) {  // four channels per thread, dealt out over the cluster
             for (int i = rank * 32 * W + tid; i < nr * (D / 4); i += ranks * 32 * W) {
-                const int k = i / (D / 4), d = (i % (D / 4)) * 4, row = row0 + k;
+                const int k = i / (D / 4), d = (i % (D / 4)) * 4, row = row0 + k, n = token(row);
                 const int32_t inv = fisr(total(s_sum, k), a.rsqrt_offset);
                 uint32_t w = 0;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w |= (uint32_t)(finish(a, total(s_o, k * OLD + d + e), inv) & 255) << (8 * e);
-                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + token(row)) * a.ldy +
-                                              (int64_t)(kvh * G + row - token(row) * G) * D + d) = w;
+                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + n) * a.ldy + (int64_t)(kvh * G + row - n * G) * D + d) = w;
             }
         };
         if (ranks == 1) {
@@ -376,7 +411,7 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     attr[1].val.clusterDim.x = grid.x;
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = grid.x > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 

@@ -508,7 +508,8 @@ typedef struct iw_tree_attn_desc {
 } iw_tree_attn_desc;
 
 /* The integer attention of iw_attention_ex for the new tokens of every
- * request over its pages. D is 64 or 128. Keys whose page number is not in
+ * request over its pages. D is 64 or 128; a page's and a row's stride are below
+ * 2^31 bytes. Keys whose page number is not in
  * [0, n_pages) or whose place is past the block table are not seen; a row that
  * sees no key gives 0, and rows from starts[B] up to N are set to 0. */
 int iw_tree_attention(const iw_tree_attn_desc *d, void *stream);
