@@ -47,6 +47,22 @@ inline cudaError_t make_tmap_2d_u8(CUtensorMap *map, const void *base, uint64_t 
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// 4-D uint8 tensor with the given sizes and strides (bytes; strides[i] steps
+// axis i+1); out-of-bounds elements of a box read as zero.
+inline cudaError_t make_tmap_4d_u8(CUtensorMap *map, const void *base, const uint64_t (&sizes)[4],
+                                   const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swz) {
+    PFN_iwEncodeTiled fn = encode_tiled_fn();
+    if (!fn) return cudaErrorNotSupported;
+    cuuint64_t dims[4] = {sizes[0], sizes[1], sizes[2], sizes[3]};
+    cuuint64_t st[3] = {strides[0], strides[1], strides[2]};
+    cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, st, bx, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // 3-D uint8 tensor: `count` windows of `rows` rows of `cols` bytes; row r of
 // window w starts at base + w*win_stride + r*ld. The row stride may be
 // smaller than a row (overlapping rows). Box [1, box_rows, box_cols], 128-byte

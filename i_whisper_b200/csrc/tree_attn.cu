@@ -8,6 +8,8 @@
 #include <cooperative_groups.h>
 
 #include "iw_common.cuh"
+#include "iw_sm100.cuh"
+#include "iw_tmap.cuh"
 #include "paged.cuh"
 
 namespace iw {
@@ -91,11 +93,15 @@ IW_DEV bool sees(const TreeAttnArgs &a, const Request &r, int t, int j) {
     return (u >> 5) < a.words && ((a.mask[(int64_t)(r.first + t) * a.words + (u >> 5)] >> (u & 31)) & 1);
 }
 
-IW_DEV int32_t finish(const TreeAttnArgs &a, int32_t acc, int32_t inv) {
-    int32_t v = rrs(wmul(acc, inv), a.rsqrt_offset);
-    v = rrs(wmul(v, inv), a.rsqrt_offset);
-    v = rrs(wmul(v, a.av_mult), a.av_shift);
-    return clampi(v, -127, 127);
+// The normalisation of one output channel.
+struct FinishK {
+    RrsK norm, out;
+    int32_t av_mult;
+};
+IW_DEV int32_t finish(const FinishK &k, int32_t acc, int32_t inv) {
+    int32_t v = rrs_apply(wmul(acc, inv), k.norm);
+    v = rrs_apply(wmul(v, inv), k.norm);
+    return clampi(rrs_apply(wmul(v, k.av_mult), k.out), -127, 127);
 }
 
 // Rows from starts[B] on are padding: the blocks of the last request zero
@@ -108,11 +114,46 @@ IW_DEV void zero_padding(const TreeAttnArgs &a, int kvh, int rank, int ranks) {
             make_int4(0, 0, 0, 0);
 }
 
+// 16-byte piece c of row `row` of a slab in shared memory lies at piece
+// swz(row, c): the 64- and 128-byte swizzles of the tensor maps, under which 8
+// consecutive rows have one piece in different banks.
+template <int D>
+IW_DEV int swz(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 3) : c ^ (row & 7); }
+
+// Loads the 32 keys from j0 of one head into a slab, completing on `bar`. TMA:
+// one box per page (or 32 rows of one) through the cache's tensor map, lane i
+// the i-th; pages of fewer than 8 rows do not fill a swizzle pattern and go
+// by 16-byte cp.async instead. Rows without a page, or past the last key's,
+// are left as they are: whatever is there is masked.
+template <int D, bool TMA>
+IW_DEV void load_slab(const TreeAttnArgs &a, const Request &r, const CUtensorMap *map, const int8_t *head, int kvh,
+                      int j0, uint8_t *dst, uint64_t *bar) {
+    const int lane = threadIdx.x & 31;
+    if (TMA) {
+        const int box = min(1 << a.page_log2, kSlab), j = j0 + lane * box;
+        const bool ok = lane * box < kSlab && has_page(a, r, j);
+        const uint32_t n = __popc(__ballot_sync(0xffffffffu, ok));
+        if (lane == 0) mbar_arrive_expect_tx(bar, n * box * D);
+        __syncwarp();
+        if (ok)
+            tma_load_4d(map, bar, dst + lane * box * D, 0, j & ((1 << a.page_log2) - 1), kvh,
+                        r.table[j >> a.page_log2]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) {
+            const int row = (e * 32 + lane) / (D / 16), c = lane % (D / 16), j = j0 + row;
+            if (has_page(a, r, j))
+                cp_async16(dst + row * D + swz<D>(row, c) * 16, head + row_at(a, r.table[j >> a.page_log2], j) + 16 * c);
+        }
+        mbar_arrive_cp_async(bar);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // Few rows per key head (single tokens, small trees): bound by reading K and V
 // once from HBM. Blocks of one to four warps, or a cluster of them, serve one
 // (request, key head) and split its keys; each warp streams slabs of 32 keys
-// through a ring of its own (cp.async, no block barrier), K first: 32 scores by
+// through a ring of its own (TMA, no block barrier), K first: 32 scores by
 // 8 rows by mma.sync with the keys as the 16-row operand, the raw scores kept in
 // shared memory so that K is not read again once the maximum over all
 // blocks is known (exchanged through distributed shared memory; the
@@ -131,33 +172,32 @@ struct Few {
     static constexpr int kRing = kStages * kSlab * D;
     static constexpr int kOutLd = D + 4;
     static size_t smem(int slots) {
-        return (size_t)W * (kRing + slots * kScoreLd * 4) + (kFewRows * kOutLd + 2 * kFewRows) * 4;
+        return 1024 + (size_t)W * (kRing + kStages * 8 + slots * kScoreLd * 4) + (kFewRows * kOutLd + 2 * kFewRows) * 4;
     }
 };
 
-// 16-byte pieces of a slab's rows are swizzled so that the fragment loads are
-// free of bank conflicts: K (one int4 per lane, two rows of 64 bytes a
-// quarter warp) needs it at 128-byte rows, V (16 rows of one piece) at both.
-template <int D>
-IW_DEV int k_piece(int row, int c) { return D == 64 ? c : c ^ ((row & 1) << 2); }
-template <int D>
-IW_DEV int v_piece(int row, int c) { return D == 64 ? c ^ ((row >> 1) & 3) : c ^ (row & 7); }
-
 // D: head dimension, W: warps per block
-template <int D, int W>
-__global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kernel(TreeAttnArgs a, int slots) {
+template <int D, int W, bool TMA>
+__global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
+    few_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                    TreeAttnArgs a, int slots) {
     namespace cg = cooperative_groups;
-    pdl_wait();
-    pdl_launch();
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_align1024(smem_raw);
     using F = Few<D, W>;
     constexpr int S = F::kStages, OLD = F::kOutLd;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + warp * F::kRing;
-    int32_t *score = reinterpret_cast<int32_t *>(smem + W * F::kRing) + warp * slots * kScoreLd;
-    int32_t *s_o = reinterpret_cast<int32_t *>(smem + W * F::kRing) + W * slots * kScoreLd;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + W * F::kRing) + warp * S;
+    int32_t *scores = reinterpret_cast<int32_t *>(smem + W * (F::kRing + S * 8));
+    int32_t *score = scores + warp * slots * kScoreLd, *s_o = scores + W * slots * kScoreLd;
     int32_t *s_sum = s_o + kFewRows * OLD, *s_max = s_sum + kFewRows;
     const int rank = blockIdx.x, ranks = gridDim.x, kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+    if (lane < S) mbar_init(&bars[lane], TMA ? 1 : 32);
+    fence_mbar_init();
+    __syncwarp();
+    pdl_wait();
+    pdl_launch();
     if (b == a.B - 1) zero_padding(a, kvh, rank, ranks);
     const Request r = request(a, b);
     const int rows = r.fresh * G;
@@ -181,26 +221,22 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
     const RrsK rk = rrs_k(a.qk_shift);
     const ExpK ek = exp_k(a.frac_bits);
 
-    for (int row0 = 0; row0 < rows; row0 += kFewRows) {
+    uint32_t base = 0;  // slabs streamed for earlier rows
+    for (int row0 = 0; row0 < rows; row0 += kFewRows, base += 2 * mine) {
         const int nr = min(kFewRows, rows - row0);
         const bool keep = mine * nr <= slots;  // otherwise the second pass computes the scores again
         auto issue = [&](int it) {             // the stream of slabs: K0 .. Kn-1, V0 .. Vn-1
-            if (it < 2 * mine) {
-                const bool v = it >= mine;
-                const int j0 = slab_at(v ? it - mine : it);
-                const int8_t *src = (v ? vbase : kbase) + 16 * (lane % (D / 16));
-                uint8_t *dst = ring + (it & (S - 1)) * (kSlab * D);
-#pragma unroll
-                for (int e = 0; e < D / 16; ++e) {
-                    const int row = (e * 32 + lane) / (D / 16), c = lane % (D / 16);
-                    const int j = min(j0 + row, r.keys - 1);  // rows past the end repeat the last: they are masked
-                    const int32_t page = r.table[j >> a.page_log2];
-                    uint8_t *to = dst + row * D + (v ? v_piece<D>(row, c) : k_piece<D>(row, c)) * 16;
-                    if (!holes || (uint32_t)page < a.n_pages) cp_async16(to, src + row_at(a, page, j));
-                    else *reinterpret_cast<int4 *>(to) = make_int4(0, 0, 0, 0);
-                }
-            }
-            cp_async_commit();
+            const int slot = (base + it) & (S - 1);
+            if (it < mine)
+                load_slab<D, TMA>(a, r, &tmap_k, kbase, kvh, slab_at(it), ring + slot * (kSlab * D), &bars[slot]);
+            else if (it < 2 * mine)
+                load_slab<D, TMA>(a, r, &tmap_v, vbase, kvh, slab_at(it - mine), ring + slot * (kSlab * D), &bars[slot]);
+        };
+        auto arrived = [&](int it) -> const uint8_t * {
+            const int slot = (base + it) & (S - 1);
+            mbar_wait(&bars[slot], ((base + it) / S) & 1);
+            __syncwarp();
+            return ring + slot * (kSlab * D);
         };
 #pragma unroll 1
         for (int i = 0; i < S; ++i) issue(i);
@@ -227,7 +263,11 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
         auto plain_slab = [&](int j0) { return !holes && j0 + kSlab <= min(r.ctx, r.keys); };
         auto on = [&](int k, int j) { return has_page(a, r, j) && sees(a, r, token(row0 + k), j); };
         int32_t m0 = INT32_MIN, m1 = INT32_MIN, mr = INT32_MIN;  // rows 2t, 2t+1 (own keys); row = lane (other slabs)
-        // raw scores of the keys 16m + g and 16m + 8 + g with all rows; load(row, h)
+        // the key of a lane's fragment rows: a quarter warp reads two rows, of 64
+        // bytes each, that must not share banks: rows g and g+1 of 64 bytes, rows
+        // that differ in bit 2 of 128 (swizzled) bytes
+        const int gk = D == 64 ? g : (g >> 1) | ((g & 1) << 2);
+        // raw scores of the keys 16m + gk and 16m + 8 + gk with all rows; load(row, h)
         // gives the lane's piece of a key's half h
         auto raw = [&](int32_t (&c)[2][4], auto load) {
 #pragma unroll
@@ -235,14 +275,14 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
                 c[m16][0] = c[m16][1] = c[m16][2] = c[m16][3] = 0;
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
-                    const int4 ka = load(16 * m16 + g, h), kb = load(16 * m16 + 8 + g, h);
+                    const int4 ka = load(16 * m16 + gk, h), kb = load(16 * m16 + 8 + gk, h);
                     mma_s8(c[m16], ka.x, kb.x, ka.y, kb.y, q[h].x, q[h].y);
                     mma_s8(c[m16], ka.z, kb.z, ka.w, kb.w, q[h].z, q[h].w);
                 }
             }
         };
         auto store = [&](int32_t *to, const int32_t (&c)[2][4]) {
-            int32_t *w = to + 2 * t * kScoreLd + g;
+            int32_t *w = to + 2 * t * kScoreLd + gk;
             if (2 * t < nr) w[0] = c[0][0], w[8] = c[0][2], w[16] = c[1][0], w[24] = c[1][2];
             if (2 * t + 1 < nr) {
                 w += kScoreLd;
@@ -253,12 +293,10 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
 #pragma unroll 1
         for (; it < mine; ++it) {
             const int j0 = slab_at(it);
-            cp_async_wait<S - 1>();
-            __syncwarp();
-            const uint8_t *ks = ring + (it & (S - 1)) * (kSlab * D);
+            const uint8_t *ks = arrived(it);
             int32_t c[2][4];
             raw(c, [&](int row, int h) {
-                return *reinterpret_cast<const int4 *>(ks + row * D + k_piece<D>(row, 4 * h + t) * 16);
+                return *reinterpret_cast<const int4 *>(ks + row * D + swz<D>(row, 4 * h + t) * 16);
             });
             const bool plain = plain_slab(j0);
             int32_t *to = score + (keep ? it * nr * kScoreLd : 0);
@@ -333,22 +371,20 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
                 __syncwarp();
                 reinterpret_cast<uint8_t *>(sc + k * kScoreLd)[lane] = (uint8_t)p;
             }
-            cp_async_wait<S - 1>();
             __syncwarp();
-            const uint8_t *vs = ring + (it & (S - 1)) * (kSlab * D) + lane * D;
+            const uint8_t *vs = arrived(it) + lane * D;
             uint32_t p0 = 0, p1 = 0;
             if (g < nr) p0 = sc[g * kScoreLd + t], p1 = sc[g * kScoreLd + 4 + t];
             sum = __dp4a(p0, 0x01010101u, __dp4a(p1, 0x01010101u, sum));
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[4];
-                ldsm_trans_b8(v, vs + v_piece<D>(lane, c) * 16);
+                ldsm_trans_b8(v, vs + swz<D>(lane, c) * 16);
                 mma_s8u8(o[c], v[0], v[1], v[2], v[3], p0, p1);
             }
             __syncwarp();
             issue(it + S);
         }
-        cp_async_wait<0>();
         // sums over the warps, then over the cluster
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -368,14 +404,15 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W) few_rows_kern
                 for (int c = 0; c < D / 16; ++c) give(d + OLD + 16 * c, o[c][1]), give(d + OLD + 16 * c + 8, o[c][3]);
             }
         }
-        auto write = [&](auto total) {  // four channels per thread, dealt out over the cluster
-            for (int i = rank * 32 * W + tid; i < nr * (D / 4); i += ranks * 32 * W) {
-                const int k = i / (D / 4), d = (i % (D / 4)) * 4, row = row0 + k, n = token(row);
+        const FinishK fk{rrs_k(a.rsqrt_offset), rrs_k(a.av_shift), a.av_mult};
+        auto write = [&](auto total) {  // two channels per thread, dealt out over the cluster
+            for (int i = rank * 32 * W + tid; i < nr * (D / 2); i += ranks * 32 * W) {
+                const int k = i / (D / 2), d = (i % (D / 2)) * 2, row = row0 + k, n = token(row);
                 const int32_t inv = fisr(total(s_sum, k), a.rsqrt_offset);
-                uint32_t w = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w |= (uint32_t)(finish(a, total(s_o, k * OLD + d + e), inv) & 255) << (8 * e);
-                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + n) * a.ldy + (int64_t)(kvh * G + row - n * G) * D + d) = w;
+                char2 w;
+                w.x = (signed char)finish(fk, total(s_o, k * OLD + d), inv);
+                w.y = (signed char)finish(fk, total(s_o, k * OLD + d + 1), inv);
+                *reinterpret_cast<char2 *>(a.y + (int64_t)(r.first + n) * a.ldy + (int64_t)(kvh * G + row - n * G) * D + d) = w;
             }
         };
         if (ranks == 1) {
@@ -415,17 +452,30 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 bloc
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int D, int W>
-static cudaError_t few_rows_launch(const TreeAttnArgs &a, int ranks, int slots, cudaStream_t st) {
+// Tensor maps of the caches: boxes of one head's rows of one page.
+struct CacheMaps {
+    CUtensorMap k, v;
+};
+static cudaError_t cache_maps(const TreeAttnArgs &a, CacheMaps &m) {
+    const uint64_t sizes[4] = {(uint64_t)a.D, 1ull << a.page_log2, (uint64_t)a.Hkv, a.n_pages};
+    const uint64_t strides[3] = {a.row_stride, (uint64_t)a.head_stride, a.page_stride};
+    const uint32_t box[4] = {(uint32_t)a.D, std::min(1u << a.page_log2, (unsigned)kSlab), 1, 1};
+    const CUtensorMapSwizzle swz = a.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    cudaError_t e = make_tmap_4d_u8(&m.k, a.k, sizes, strides, box, swz);
+    return e == cudaSuccess ? make_tmap_4d_u8(&m.v, a.v, sizes, strides, box, swz) : e;
+}
+
+template <int D, int W, bool TMA>
+static cudaError_t few_rows_launch(const TreeAttnArgs &a, const CacheMaps &m, int ranks, int slots, cudaStream_t st) {
     const size_t smem = Few<D, W>::smem(slots);
     static SmemLimit lim;
-    cudaError_t e = raise_smem_limit(few_rows_kernel<D, W>, smem, lim);
+    cudaError_t e = raise_smem_limit(few_rows_kernel<D, W, TMA>, smem, lim);
     if (e != cudaSuccess) return e;
-    return launch_cluster(few_rows_kernel<D, W>, dim3(ranks, a.Hkv, a.B), dim3(32 * W), smem, st, a, slots);
+    return launch_cluster(few_rows_kernel<D, W, TMA>, dim3(ranks, a.Hkv, a.B), dim3(32 * W), smem, st, m.k, m.v, a, slots);
 }
 
 template <int D>
-static cudaError_t few_rows(const TreeAttnArgs &a, cudaStream_t st) {
+static cudaError_t few_rows(const TreeAttnArgs &a, const CacheMaps &m, bool tma, cudaStream_t st) {
     const int64_t keys = std::max<int64_t>(1, (int64_t)a.width << a.page_log2), pairs = (int64_t)a.B * a.Hkv;
     // One warp per (request, key head) needs no barrier and shares no sums; more
     // warps, then more blocks, while the SMs have fewer than 16 warps each and a
@@ -441,16 +491,23 @@ static cudaError_t few_rows(const TreeAttnArgs &a, cudaStream_t st) {
     const int64_t per_warp = (keys / kSlab / ranks + W) / W;
     const int64_t guess = std::min<int64_t>(kFewRows, std::max<int64_t>(1, (a.N + a.B - 1) / a.B * a.G));
     const int slots = (int)std::min<int64_t>(64, std::max<int64_t>(kFewRows, per_warp * guess));
-    if (W == 1) return few_rows_launch<D, 1>(a, ranks, slots, st);
-    if (W == 2) return few_rows_launch<D, 2>(a, ranks, slots, st);
-    return few_rows_launch<D, 4>(a, ranks, slots, st);
+    if (!tma) return few_rows_launch<D, 4, false>(a, m, ranks, slots, st);
+    if (W == 1) return few_rows_launch<D, 1, true>(a, m, ranks, slots, st);
+    if (W == 2) return few_rows_launch<D, 2, true>(a, m, ranks, slots, st);
+    return few_rows_launch<D, 4, true>(a, m, ranks, slots, st);
 }
 
 }  // namespace tree
 
 cudaError_t tree_attention(const TreeAttnArgs &a, cudaStream_t st) {
     if (a.B == 0) return cudaMemset2DAsync(a.y, a.ldy, 0, (size_t)a.H * a.D, (size_t)a.N, st);
-    return a.D == 64 ? tree::few_rows<64>(a, st) : tree::few_rows<128>(a, st);
+    // pages of 8 rows and more go through tensor maps
+    // tensor maps need pages of 8 rows or more and axes that step
+    const bool tma = a.page_log2 >= 3 && a.n_pages > 0 && a.row_stride > 0 && a.head_stride > 0 && a.page_stride > 0;
+    tree::CacheMaps m = {};
+    if (tma)
+        if (cudaError_t e = tree::cache_maps(a, m); e != cudaSuccess) return e;
+    return a.D == 64 ? tree::few_rows<64>(a, m, tma, st) : tree::few_rows<128>(a, m, tma, st);
 }
 
 }  // namespace iw
