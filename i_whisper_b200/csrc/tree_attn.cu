@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
     const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, b = blockIdx.z, G = a.G;
     if (lane < S) mbar_init(&bars[lane], TMA ? 1 : 32);
     fence_mbar_init();
+    if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     __syncwarp();
     pdl_wait();
     pdl_launch();
