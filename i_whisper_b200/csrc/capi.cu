@@ -777,7 +777,7 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
     if (!d) return fail(IW_EINVAL, "iw_tree_attention: null descriptor");
     if (d->B < 0 || d->B > 65535 || d->N < 0 || d->N > INT32_MAX || d->H < 1 || d->H > 4096 || d->Hkv < 1 || d->n_pages < 0 ||
         d->n_pages > INT32_MAX || d->table_width < 0 || d->table_ld < d->table_width || d->mask_words < 0 ||
-        d->mask_words > IW_PLAN_MAX_REQUESTS)
+        d->mask_words > IW_PLAN_MAX_REQUESTS || d->N * d->H > INT32_MAX)
         return fail(IW_EINVAL, "iw_tree_attention: invalid shape");
     if (d->H % d->Hkv) return fail(IW_EINVAL, "iw_tree_attention: the head count must be a multiple of the key head count");
     if (d->D != 64 && d->D != 128) return fail(IW_EINVAL, "iw_tree_attention: head dimension must be 64 or 128");

@@ -21,7 +21,7 @@ struct Slab {
     static constexpr int kKeys = 4096 / D;
 };
 
-// c += a (16 rows x 32, signed bytes) * b (32 x 8 bytes, signed or unsigned).
+// c += a (16 rows x 32 bytes) * b (32 x 8 bytes), either signed or unsigned.
 // Lane (g = lane/4, t = lane%4) holds a0/a1: rows g/g+8, k 4t..4t+3, a2/a3:
 // the same rows, k 16+4t..; b0/b1: column g, k 4t.. / 16+4t..; c0,c1/c2,c3:
 // rows g/g+8, columns 2t, 2t+1.
@@ -32,6 +32,11 @@ IW_DEV void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint3
 }
 IW_DEV void mma_s8u8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+IW_DEV void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -137,30 +142,37 @@ IW_DEV void load_boxes(const TreeAttnArgs &a, const CUtensorMap *map, int kvh, i
     if (ok)
         tma_load_4d(map, bar, dst + lane * box * D, 0, (j0 + lane * box) & ((1 << a.page_log2) - 1), kvh, page);
 }
-template <int D>
+template <int D, int BYTES>
 IW_DEV void load_rows(const TreeAttnArgs &a, const Request &r, const int8_t *head, int j0, uint8_t *dst, uint64_t *bar) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < BYTES / 512; ++e) {
         const int row = (e * 32 + lane) / (D / 16), c = lane % (D / 16), j = j0 + row;
         if (has_page(a, r, j))
             cp_async16(dst + row * D + swz<D>(row, c) * 16, head + row_at(a, r.table[j >> a.page_log2], j) + 16 * c);
     }
     mbar_arrive_cp_async(bar);
 }
-// Bounded wait for a slab; a wait that gives up sets the device status word.
-IW_DEV void slab_wait(uint64_t *bar, uint32_t parity) {
-    uint64_t t0 = 0;
-    for (uint32_t i = 1; !mbar_try_wait_suspend(bar, parity, 200000u); ++i)
-        if ((i & 63u) == 0) {
-            if (t0 == 0) t0 = globaltimer_ns();
-            else if (globaltimer_ns() - t0 > g_wait_timeout_ns) {
-                atomicOr(&g_device_status, IW_DEVERR_WAIT_TIMEOUT);
-                break;
+// Bounded wait of a warp for a slab. A wait that gives up sets the device
+// status word, and this warp's later waits then give up after a millisecond each,
+// so that the kernel ends soon and with its copies landed.
+struct SlabWait {
+    bool late = false;
+    IW_DEV void operator()(uint64_t *bar, uint32_t parity) {
+        uint64_t t0 = 0;
+        for (uint32_t i = 1; !mbar_try_wait_suspend(bar, parity, 200000u); ++i)
+            if ((i & 63u) == 0) {
+                if (t0 == 0) {
+                    t0 = globaltimer_ns();
+                } else if (globaltimer_ns() - t0 > (late ? 1000000ull : g_wait_timeout_ns)) {
+                    atomicOr(&g_device_status, IW_DEVERR_WAIT_TIMEOUT);
+                    late = true;
+                    break;
+                }
             }
-        }
-    __syncwarp();
-}
+        __syncwarp();
+    }
+};
 
 // ---------------------------------------------------------------------------
 // Few rows per key head (single tokens, small trees): bound by reading K and V
@@ -250,6 +262,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
     const FinishK fk{rrs_k(a.rsqrt_offset), rrs_k(a.av_shift), a.av_mult};
     auto requant = [&](int32_t acc) { return clampi(rrs_apply(wmul(acc, a.qk_mult), rk), -32768, 32767); };
 
+    SlabWait slab_wait;
     uint32_t base = 0;  // slabs streamed for earlier rows
     for (int row0 = first_row; row0 < rows; row0 += row_step, base += 2 * mine) {
         const int nr = NR == 1 ? 1 : min(group, rows - row0);
@@ -265,7 +278,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
                 load_boxes<D>(a, v ? &tmap_v : &tmap_k, kvh, j0, box, page, lane < per && page >= 0, ring + slot * 4096,
                               &bars[slot]);
             } else {
-                load_rows<D>(a, r, v ? vbase : kbase, j0, ring + slot * 4096, &bars[slot]);
+                load_rows<D, 4096>(a, r, v ? vbase : kbase, j0, ring + slot * 4096, &bars[slot]);
             }
         };
         auto arrived = [&](int it) -> const uint8_t * {
@@ -509,6 +522,363 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows per key head (trees, prompts, shared key heads): bound by the
+// arithmetic of the integer softmax and the score products. A block, or a
+// cluster of them that splits the keys, serves one (request, key head); four
+// warps compute, a fifth feeds a ring of 64-key K and V tiles by TMA (a full
+// and an empty barrier per tile). A warp holds 16 rows: scores by mma.sync, the
+// keys of a tile in such an order that a thread's four probabilities are four
+// consecutive operand bytes of P.V, which therefore never leave registers; V
+// transposed by ldmatrix. The maximum needs all keys before the first
+// probability, so K is read twice (the second time from L2) and its products
+// taken twice: keeping 16 rows of scores would take more shared memory than the
+// K that they come from. Warps share a tile between up to four groups of 16
+// rows; with fewer groups they divide the tiles. tcgen05 would hold scores in
+// tensor memory, from where the softmax has to fetch them, and it wants 128
+// rows, which trees of 64 tokens on one head do not have.
+// ---------------------------------------------------------------------------
+constexpr int kManyWarps = 4, kTile = 64;
+
+template <int D>
+struct Many {
+    static constexpr int kStages = 8;
+    static constexpr int kBytes = kTile * D;
+    static constexpr int kOutLd = D + 4;
+    static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * (kOutLd + 2) * 4; }
+};
+
+// The probability of a score from its raw sum, all in the FMA pipe but for a
+// select and a mask (the ALU pipe issues at half its rate). d = x - M - 1 with
+// 12582912 added, so that its bits are also the float 1.5 * 2^23 + d; floors of
+// d/2 and d/16 are fused multiply-adds rounded down, f = d + floor(d/2) - floor(d/16)
+// is exact, and the bits of 2^(7 + xi) * (1 + fr / 2^(fb+1)), f = xi * 2^fb + fr,
+// follow by two integer multiply-adds; its whole part is the probability.
+// Valid for 7 to 14 fraction bits, shifts 2 to 30 and rows whose maximum and
+// cut-off lie inside 16 bits (so that the clamps of x change nothing).
+struct FastExp {
+    int32_t mult, rnd, up, limit, below, mask, scale, zero, half;
+};
+constexpr int32_t kBias = 0x4B400000;  // bits of 12582912.0f
+IW_DEV FastExp fast_exp(const TreeAttnArgs &a) {
+    const int fb = min(max(a.frac_bits, 7), 14), s = (int)min(max(a.qk_shift, 2u), 30u);
+    FastExp k;
+    k.mult = a.qk_mult;
+    k.rnd = 1 << (s - 1);
+    k.up = 1 << (32 - s);
+    k.limit = kBias - min(22795, 8 << fb);
+    k.below = kBias - (8 << fb);
+    k.mask = (1 << fb) - 1;
+    k.scale = 1 << (23 - fb);
+    k.zero = (int32_t)((134u << 23) - ((uint32_t)kBias << (23 - fb)));
+    k.half = -(1 << (22 - fb));
+    return k;
+}
+// `base` = kBias - M - 1; the result's low byte is the probability.
+IW_DEV uint32_t fast_prob(int32_t acc, int32_t base, const FastExp &k) {
+    int32_t t = acc * k.mult + k.rnd, d;
+    asm("mad.hi.s32 %0, %1, 1, %2;" : "=r"(t) : "r"(acc), "r"(t));        // halves away from zero
+    asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(t), "r"(k.up), "r"(base));  // (t >> s) + base
+    d = d < k.limit ? k.below : d;
+    const float x = __int_as_float(d);
+    const float f = __fadd_rn(x, __fadd_rn(__fmaf_rd(x, 0.5f, 6291456.f), -__fmaf_rd(x, 0.0625f, 11796480.f)));
+    const int32_t bits = __float_as_int(f);
+    const int32_t w = (bits & k.mask) * k.half + (bits * k.scale + k.zero);
+    return __float_as_uint(__fadd_rz(__int_as_float(w), 8388608.f));
+}
+
+template <int D, bool TMA>
+__global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
+    many_rows_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                     TreeAttnArgs a, int ranks) {
+    namespace cg = cooperative_groups;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_align1024(smem_raw);
+    using F = Many<D>;
+    constexpr int S = F::kStages, OLD = F::kOutLd;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * F::kBytes), *empty = full + S;
+    int32_t *s_o = reinterpret_cast<int32_t *>(empty + S), *s_sum = s_o + 64 * OLD, *s_max = s_sum + 64;
+    const int lr = 31 - __clz(ranks);  // a power of two
+    const int rank = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+    if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
+    pdl_wait();
+    pdl_launch();
+    if (b == a.B - 1) zero_padding(a, kvh, rank, ranks);
+    const Request r = request(a, b);
+    const int rows = r.fresh * G;
+    if (rows == 0) return;
+    // RT groups of 16 rows side by side, KG sets of warps that share out the tiles:
+    // set i takes tiles i, i + KG, ... through SG slots of the ring that are its own (a
+    // set has to see every phase of the barriers it waits on)
+    const int lrt = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2), lkg = 2 - lrt, lsg = 3 - lkg;
+    static_assert(kManyWarps == 4 && S == 8, "powers of two above");
+    const int RT = 1 << lrt, KG = 1 << lkg, SG = 1 << lsg;
+    if (tid < S) {
+        mbar_init(&full[tid], TMA ? 1 : 32);
+        mbar_init(&empty[tid], RT);
+    }
+    fence_mbar_init();
+    __syncthreads();
+    const int tiles = (r.keys + kTile - 1) / kTile;
+    const int first = (tiles * rank) >> lr, mine = ((tiles * (rank + 1)) >> lr) - first;
+    cg::cluster_group cl = cg::this_cluster();
+    SlabWait slab_wait;
+
+    if (warp == kManyWarps) {  // the feeder: K tiles, then K and V tiles in turn, for every block of rows
+        const int8_t *kbase = a.k + kvh * a.head_stride, *vbase = a.v + kvh * a.head_stride;
+        const int box = min(1 << a.page_log2, kTile);
+        uint32_t done = 0;  // blocks of rows fed
+        auto put = [&](bool pass2, bool v, int i) {
+            const uint32_t set = i & (KG - 1), at = i >> lkg, count = (mine - set + KG - 1) >> lkg;
+            const uint32_t n = 3 * count * done + (pass2 ? count + 2 * at + v : at), slot = (set << lsg) + (n & (SG - 1));
+            if (n >= SG) slab_wait(&empty[slot], ((n >> lsg) - 1) & 1);
+            const int j0 = (first + i) * kTile;
+            uint8_t *dst = smem + slot * F::kBytes;
+            if (TMA) {
+                const int j = j0 + lane * box;
+                const int32_t page = lane * box < kTile && j < r.keys ? r.table[j >> a.page_log2] : -1;
+                load_boxes<D>(a, v ? &tmap_v : &tmap_k, kvh, j0, box, page, (uint32_t)page < a.n_pages, dst, &full[slot]);
+            } else {
+                load_rows<D, F::kBytes>(a, r, v ? vbase : kbase, j0, dst, &full[slot]);
+            }
+        };
+        for (int row0 = 0; row0 < rows; row0 += 16 * RT, ++done) {
+            for (int i = 0; i < mine; ++i) put(false, false, i);
+            // a ring of the second pass's tiles goes out before the blocks meet
+            const int ahead = min(S, 2 * mine);
+            for (int i = 0; i < ahead; ++i) put(true, i & 1, i >> 1);
+            if (ranks > 1) cl.sync();
+            for (int i = ahead; i < 2 * mine; ++i) put(true, i & 1, i >> 1);
+            if (ranks > 1) cl.sync(), cl.sync();
+        }
+        return;
+    }
+
+    const int rt = warp & (RT - 1), kg = warp >> lrt;
+    const RrsK rk = rrs_k(a.qk_shift);
+    const FastExp fx = fast_exp(a);
+    const FinishK fk{rrs_k(a.rsqrt_offset), rrs_k(a.av_shift), a.av_mult};
+    const bool fast_ok = a.frac_bits >= 7 && a.frac_bits <= 14 && a.qk_shift >= 2 && a.qk_shift <= 30;
+    const int cut = min(22795, 8 << min(max(a.frac_bits, 7), 14));
+    auto requant = [&](int32_t acc) { return clampi(rrs_apply(wmul(acc, a.qk_mult), rk), -32768, 32767); };
+    auto meet = [&] {
+        if (ranks > 1) cl.sync();
+        else asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");
+    };
+    // the key, of 16, whose row a lane loads for column n = 2t'+e of score tile jj:
+    // operand byte 4t' + 2jj + e of P is that of key order(4t' + 2jj + e). 128-byte
+    // rows need another order than 64-byte ones so that neither the K nor the V
+    // fragments meet bank conflicts
+    auto order = [](int k) { return D == 64 ? k : 8 * (k >> 3) + 4 * (k & 1) + 2 * ((k >> 1) & 1) + ((k >> 2) & 1); };
+    const int krow0 = order(4 * (g >> 1) + (g & 1)), krow1 = order(4 * (g >> 1) + 2 + (g & 1));
+    const int vrow = (lane & 16) + order(lane & 15);
+
+    uint32_t n = 0;  // tiles of this set's slots seen so far
+    auto slot = [&](uint32_t n) { return (kg << lsg) + (n & (SG - 1)); };
+    auto tile_at = [&](uint32_t n) { return smem + slot(n) * F::kBytes; };
+    auto arrived = [&](uint32_t n) { slab_wait(&full[slot(n)], (n >> lsg) & 1); };
+    auto release = [&](uint32_t n) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot(n)]);
+    };
+    for (int row0 = 0; row0 < rows; row0 += 16 * RT) {
+        const int ra = row0 + 16 * rt + g, rb = ra + 8;  // this lane's rows
+        const int ta = G == 1 ? ra : ra / G, tb = G == 1 ? rb : rb / G;
+        int4 q0[D / 64], q1[D / 64];
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+            q0[c] = q1[c] = make_int4(0, 0, 0, 0);
+            if (ra < rows)
+                q0[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + ta) * a.ldq +
+                                                        (int64_t)(kvh * G + ra - ta * G) * a.q_hs + 64 * c + 16 * t);
+            if (rb < rows)
+                q1[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + tb) * a.ldq +
+                                                        (int64_t)(kvh * G + rb - tb * G) * a.q_hs + 64 * c + 16 * t);
+        }
+        for (int i = tid; i < 64 * (OLD + 2); i += 32 * kManyWarps) s_o[i] = i < 64 * OLD + 64 ? 0 : INT32_MIN;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");
+
+        // which keys j0 .. j0+31 the rows ra and rb see; true when all of them by all
+        auto seen = [&](int j0, uint32_t &wa, uint32_t &wb) {
+            const uint32_t there = __ballot_sync(0xffffffffu, has_page(a, r, j0 + lane));
+            wa = wb = there;
+            if (j0 + 32 <= r.ctx) return there == 0xffffffffu;
+            const int u0 = j0 - r.ctx;  // place of the first key among the new tokens
+            auto word = [&](int n) -> uint32_t {
+                if (a.words == 0) return n < u0 ? 0u : (n - u0 >= 31 ? 0xffffffffu : (2u << (n - u0)) - 1);
+                if (n >= r.fresh) return 0;
+                const int32_t *m = a.mask + (int64_t)(r.first + n) * a.words;
+                auto at = [&](int w) -> uint32_t { return w < 0 ? 0xffffffffu : (w < a.words ? (uint32_t)m[w] : 0u); };
+                return __funnelshift_r(at(u0 >> 5), at((u0 >> 5) + 1), u0 & 31);
+            };
+            wa &= word(ta);
+            wb &= word(tb);
+            return false;
+        };
+        // raw scores of 32 keys: c[2 * half + jj], columns order(4t + 2jj + e) + 16 * half
+        auto raw = [&](int32_t (&c)[4][4], const uint8_t *ks) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int row = 16 * (j >> 1) + ((j & 1) ? krow1 : krow0);
+                c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0;
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) {
+                    const int4 k = *reinterpret_cast<const int4 *>(ks + row * D + swz<D>(row, 4 * h + t) * 16);
+                    mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
+                    mma_s8(c[j], q0[h].z, q1[h].z, q0[h].w, q1[h].w, k.z, k.w);
+                }
+            }
+        };
+        auto bit = [&](int j, int e) { return 16 * (j >> 1) + order(4 * t + 2 * (j & 1) + e); };
+
+        int32_t m0 = INT32_MIN, m1 = INT32_MIN;
+        for (int i = kg; i < mine; i += KG, ++n) {
+            arrived(n);
+#pragma unroll
+            for (int h32 = 0; h32 < kTile / 32; ++h32) {
+                int32_t c[4][4];
+                raw(c, tile_at(n) + h32 * 32 * D);
+                uint32_t wa, wb;
+                if (!seen((first + i) * kTile + 32 * h32, wa, wb)) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if (!((wa >> bit(j, e)) & 1)) c[j][e] = INT32_MIN;
+                            if (!((wb >> bit(j, e)) & 1)) c[j][2 + e] = INT32_MIN;
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    m0 = max(m0, max(c[j][0], c[j][1]));
+                    m1 = max(m1, max(c[j][2], c[j][3]));
+                }
+            }
+            release(n);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            m0 = max(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+            m1 = max(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+        }
+        if (t == 0) atomicMax(&s_max[16 * rt + g], m0), atomicMax(&s_max[16 * rt + g + 8], m1);
+        meet();
+        if (ranks == 1) {
+            m0 = s_max[16 * rt + g];
+            m1 = s_max[16 * rt + g + 8];
+        } else {
+            for (int k = 0; k < ranks; ++k) {
+                const int32_t *o = cl.map_shared_rank(s_max, k);
+                m0 = max(m0, o[16 * rt + g]);
+                m1 = max(m1, o[16 * rt + g + 8]);
+            }
+        }
+        const int32_t xa = (m0 == INT32_MIN ? -32768 : requant(m0)) + 1, xb = (m1 == INT32_MIN ? -32768 : requant(m1)) + 1;
+        auto inside = [&](int32_t xm) { return xm <= 32767 && xm - cut >= -32768; };
+        const bool fast = __all_sync(0xffffffffu, fast_ok && (ra >= rows || inside(xa)) && (rb >= rows || inside(xb)));
+
+        int32_t o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0;
+        uint32_t sum0 = 0, sum1 = 0;
+        for (int i = kg; i < mine; i += KG, n += 2) {
+            uint32_t p[kTile / 32][4];
+            arrived(n);
+#pragma unroll
+            for (int h32 = 0; h32 < kTile / 32; ++h32) {
+                int32_t c[4][4];
+                raw(c, tile_at(n) + h32 * 32 * D);
+                if (fast) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[j][e] = (int32_t)fast_prob(c[j][e], kBias - (e < 2 ? xa : xb), fx);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            c[j][e] = shift_exp_one(requant(c[j][e]), (int16_t)(e < 2 ? xa : xb), a.frac_bits);
+                }
+                auto pack = [](int32_t x, int32_t y, int32_t z, int32_t w) {
+                    return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+                };
+                uint32_t (&a4)[4] = p[h32];
+                a4[0] = pack(c[0][0], c[0][1], c[1][0], c[1][1]);
+                a4[1] = pack(c[0][2], c[0][3], c[1][2], c[1][3]);
+                a4[2] = pack(c[2][0], c[2][1], c[3][0], c[3][1]);
+                a4[3] = pack(c[2][2], c[2][3], c[3][2], c[3][3]);
+                uint32_t wa, wb;
+                if (!seen((first + i) * kTile + 32 * h32, wa, wb)) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t w = (x & 1) ? wb : wa;
+                        uint32_t keep = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if ((w >> (16 * (x >> 1) + order(4 * t + e))) & 1) keep |= 0xffu << (8 * e);
+                        a4[x] &= keep;
+                    }
+                }
+                sum0 = __dp4a(a4[0], 0x01010101u, __dp4a(a4[2], 0x01010101u, sum0));
+                sum1 = __dp4a(a4[1], 0x01010101u, __dp4a(a4[3], 0x01010101u, sum1));
+            }
+            release(n);
+            arrived(n + 1);
+            const uint8_t *vs = tile_at(n + 1);
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+                for (int h32 = 0; h32 < kTile / 32; ++h32) {
+                    const int row = 32 * h32 + vrow;
+                    uint32_t v[4];
+                    ldsm_trans_b8(v, vs + row * D + swz<D>(row, c) * 16);
+                    mma_u8s8(o[2 * c], p[h32][0], p[h32][1], p[h32][2], p[h32][3], v[0], v[2]);
+                    mma_u8s8(o[2 * c + 1], p[h32][0], p[h32][1], p[h32][2], p[h32][3], v[1], v[3]);
+                }
+            release(n + 1);
+        }
+        // sums over the warps that shared the tiles, then over the cluster
+        sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, 1);
+        sum0 += __shfl_xor_sync(0xffffffffu, sum0, 2);
+        sum1 += __shfl_xor_sync(0xffffffffu, sum1, 2);
+        auto give = [&](int32_t *d, int32_t v) {
+            if (KG > 1) atomicAdd(d, v);
+            else *d = v;
+        };
+        if (t == 0) give(&s_sum[16 * rt + g], (int32_t)sum0), give(&s_sum[16 * rt + g + 8], (int32_t)sum1);
+        int32_t *d0 = s_o + (16 * rt + g) * OLD + 2 * t;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+            give(d0 + 8 * c, o[c][0]), give(d0 + 8 * c + 1, o[c][1]);
+            give(d0 + 8 * OLD + 8 * c, o[c][2]), give(d0 + 8 * OLD + 8 * c + 1, o[c][3]);
+        }
+        meet();
+        auto total = [&](int32_t *p, int i) {
+            if (ranks == 1) return p[i];
+            uint32_t v = 0;
+            for (int k = 0; k < ranks; ++k) v += (uint32_t)cl.map_shared_rank(p, k)[i];
+            return (int32_t)v;
+        };
+        // one row per warp and step, two channels per lane
+        for (int k = rank * kManyWarps + warp; k < min(16 * RT, rows - row0); k += ranks * kManyWarps) {
+            const int row = row0 + k, tok = row / G;
+            const int32_t inv = fisr(total(s_sum, k), a.rsqrt_offset);
+            int8_t *out = a.y + (int64_t)(r.first + tok) * a.ldy + (int64_t)(kvh * G + row - tok * G) * D;
+#pragma unroll
+            for (int d = 2 * lane; d < D; d += 64) {
+                char2 w;
+                w.x = (signed char)finish(fk, total(s_o, k * OLD + d), inv);
+                w.y = (signed char)finish(fk, total(s_o, k * OLD + d + 1), inv);
+                *reinterpret_cast<char2 *>(out + d) = w;
+            }
+        }
+        meet();  // no block's sums go away or are cleared while another reads them
+    }
+}
+
 // Kernel launch with clusters of `ranks` blocks along x and the PDL attribute.
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_cluster(void (*kernel)(KArgs...), int ranks, dim3 grid, dim3 block, size_t smem,
@@ -533,10 +903,10 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), int ranks, dim3 grid
 struct CacheMaps {
     CUtensorMap k, v;
 };
-static cudaError_t cache_maps(const TreeAttnArgs &a, CacheMaps &m) {
+static cudaError_t cache_maps(const TreeAttnArgs &a, int rows, CacheMaps &m) {
     const uint64_t sizes[4] = {(uint64_t)a.D, 1ull << a.page_log2, (uint64_t)a.Hkv, a.n_pages};
     const uint64_t strides[3] = {a.row_stride, (uint64_t)a.head_stride, a.page_stride};
-    const uint32_t box[4] = {(uint32_t)a.D, std::min(1u << a.page_log2, 4096u / a.D), 1, 1};
+    const uint32_t box[4] = {(uint32_t)a.D, std::min(1u << a.page_log2, (unsigned)rows), 1, 1};
     const CUtensorMapSwizzle swz = a.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     cudaError_t e = make_tmap_4d_u8(&m.k, a.k, sizes, strides, box, swz);
     return e == cudaSuccess ? make_tmap_4d_u8(&m.v, a.v, sizes, strides, box, swz) : e;
@@ -591,17 +961,40 @@ static cudaError_t few_rows(const TreeAttnArgs &a, const CacheMaps &m, bool tma,
     return p.group == 1 ? few_rows_warps<D, 1>(a, m, tma, p, st) : few_rows_warps<D, kFewRows>(a, m, tma, p, st);
 }
 
+template <int D, bool TMA>
+static cudaError_t many_rows(const TreeAttnArgs &a, const CacheMaps &m, cudaStream_t st) {
+    const int64_t keys = std::max<int64_t>(1, (int64_t)a.width << a.page_log2), pairs = (int64_t)a.B * a.Hkv;
+    // split the keys while there are fewer than four blocks per SM and a block
+    // keeps 256 keys
+    int ranks = 1;
+    while (ranks < 8 && pairs * ranks < 4 * num_sms() && keys / ranks > 256) ranks *= 2;
+    const size_t smem = Many<D>::smem();
+    static SmemLimit lim;
+    cudaError_t e = raise_smem_limit(many_rows_kernel<D, TMA>, smem, lim);
+    if (e != cudaSuccess) return e;
+    return launch_cluster(many_rows_kernel<D, TMA>, ranks, dim3(ranks, a.Hkv, a.B), dim3(32 * (kManyWarps + 1)), smem, st,
+                          m.k, m.v, a, ranks);
+}
+
+template <int D>
+static cudaError_t attention(const TreeAttnArgs &a, cudaStream_t st) {
+    // tensor maps need pages of 8 rows or more and axes that step
+    const bool tma = a.page_log2 >= 3 && a.n_pages > 0 && a.row_stride > 0 && a.head_stride > 0 && a.page_stride > 0;
+    // the batch's mean decides for all of it; either kernel takes any count
+    const int64_t mean_rows = (a.N + a.B - 1) / a.B * a.G;
+    const bool many = mean_rows > kFewRows;
+    CacheMaps m = {};
+    if (tma)
+        if (cudaError_t e = cache_maps(a, many ? kTile : Slab<D>::kKeys, m); e != cudaSuccess) return e;
+    if (!many) return few_rows<D>(a, m, tma, mean_rows, st);
+    return tma ? many_rows<D, true>(a, m, st) : many_rows<D, false>(a, m, st);
+}
+
 }  // namespace tree
 
 cudaError_t tree_attention(const TreeAttnArgs &a, cudaStream_t st) {
     if (a.B == 0) return cudaMemset2DAsync(a.y, a.ldy, 0, (size_t)a.H * a.D, (size_t)a.N, st);
-    // tensor maps need pages of 8 rows or more and axes that step
-    const bool tma = a.page_log2 >= 3 && a.n_pages > 0 && a.row_stride > 0 && a.head_stride > 0 && a.page_stride > 0;
-    tree::CacheMaps m = {};
-    if (tma)
-        if (cudaError_t e = tree::cache_maps(a, m); e != cudaSuccess) return e;
-    const int64_t mean_rows = (a.N + a.B - 1) / a.B * a.G;
-    return a.D == 64 ? tree::few_rows<64>(a, m, tma, mean_rows, st) : tree::few_rows<128>(a, m, tma, mean_rows, st);
+    return a.D == 64 ? tree::attention<64>(a, st) : tree::attention<128>(a, st);
 }
 
 }  // namespace iw
