@@ -35,19 +35,25 @@ IW_DEV void mma_s8u8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uin
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-IW_DEV void mma_u8s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// c = a * b, signed.
+IW_DEV void mma_s8_first(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 // Two 16 x 16 byte tiles, transposed: lanes 0-15 point at the rows of the
 // first, 16-31 at those of the second; r0/r1: rows 4t..4t+3 of columns g / 8+g
 // of the first tile, r2/r3 of the second.
-IW_DEV void ldsm_trans_b8(uint32_t (&r)[4], const void *p) {
+IW_DEV void ldsm_trans_b8(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"((uint32_t)__cvta_generic_to_shared(p))
+                 : "r"(at)
                  : "memory");
+}
+IW_DEV int4 lds_v4(uint32_t at) {
+    int4 v;
+    asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
 }
 
 // Raw scores of a slab: accumulators of its 16-key tiles.
@@ -465,7 +471,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
                 for (int e = 0; e < SL / 32; ++e) {
                     const int row = 32 * e + lane;
                     uint32_t v[4];
-                    ldsm_trans_b8(v, vs + row * D + swz<D>(row, c) * 16);
+                    ldsm_trans_b8(v, smem_u32(vs) + row * D + swz<D>(row, c) * 16);
                     mma_s8u8(o[c], v[0], v[1], v[2], v[3], p[2 * e], p[2 * e + 1]);
                 }
             __syncwarp();
@@ -548,24 +554,26 @@ struct Many {
     static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * (kOutLd + 2) * 4; }
 };
 
-// The probability of a score from its raw sum, all in the FMA pipe but for a
-// select and a mask (the ALU pipe issues at half its rate). d = x - M - 1 with
-// 12582912 added, so that its bits are also the float 1.5 * 2^23 + d; floors of
-// d/2 and d/16 are fused multiply-adds rounded down, f = d + floor(d/2) - floor(d/16)
-// is exact, and the bits of 2^(7 + xi) * (1 + fr / 2^(fb+1)), f = xi * 2^fb + fr,
-// follow by two integer multiply-adds; its whole part is the probability.
-// Valid for 7 to 14 fraction bits, shifts 2 to 30 and rows whose maximum and
-// cut-off lie inside 16 bits (so that the clamps of x change nothing).
+// The probability of a score from its raw sum, mostly in the FMA pipe (the ALU
+// pipe issues at half its rate). One wide multiply-add and a shift give
+// d = x - M - 1: the multiplier m * 2^22 + 1 adds the sum itself, less than
+// 2^22, below the product's last place, which rounds halves away from zero. d
+// comes with 12582912 added, so that its bits are also the float
+// 1.5 * 2^23 + d; floors of d/2 and d/16 are fused multiply-adds rounded down,
+// f = d + floor(d/2) - floor(d/16) is exact, and the bits of
+// 2^(7 + xi) * (1 + fr / 2^(fb+1)), f = xi * 2^fb + fr, follow by two integer
+// multiply-adds; its whole part is the probability. Valid for 7 to 14
+// fraction bits, shifts 1 to 9 and rows whose maximum and cut-off lie inside 16
+// bits (so that the clamps of x change nothing).
 struct FastExp {
-    int32_t mult, rnd, up, limit, below, mask, scale, zero, half;
+    int32_t mult, shift, limit, below, mask, scale, zero, half;
 };
 constexpr int32_t kBias = 0x4B400000;  // bits of 12582912.0f
 IW_DEV FastExp fast_exp(const TreeAttnArgs &a) {
-    const int fb = min(max(a.frac_bits, 7), 14), s = (int)min(max(a.qk_shift, 2u), 30u);
+    const int fb = min(max(a.frac_bits, 7), 14);
     FastExp k;
-    k.mult = a.qk_mult;
-    k.rnd = 1 << (s - 1);
-    k.up = 1 << (32 - s);
+    k.mult = (a.qk_mult << 22) + 1;
+    k.shift = 22 + (int)min(a.qk_shift, 9u);
     k.limit = kBias - min(22795, 8 << fb);
     k.below = kBias - (8 << fb);
     k.mask = (1 << fb) - 1;
@@ -574,11 +582,13 @@ IW_DEV FastExp fast_exp(const TreeAttnArgs &a) {
     k.half = -(1 << (22 - fb));
     return k;
 }
-// `base` = kBias - M - 1; the result's low byte is the probability.
-IW_DEV uint32_t fast_prob(int32_t acc, int32_t base, const FastExp &k) {
-    int32_t t = acc * k.mult + k.rnd, d;
-    asm("mad.hi.s32 %0, %1, 1, %2;" : "=r"(t) : "r"(acc), "r"(t));        // halves away from zero
-    asm("mad.hi.s32 %0, %1, %2, %3;" : "=r"(d) : "r"(t), "r"(k.up), "r"(base));  // (t >> s) + base
+// A row's addend for maximum + 1 = xm.
+IW_DEV int64_t fast_base(int32_t xm, const FastExp &k) {
+    return ((int64_t)(kBias - xm) << k.shift) + ((int64_t)1 << (k.shift - 1));
+}
+IW_DEV uint32_t fast_prob(int32_t acc, int64_t base, const FastExp &k) {
+    const int64_t t = (int64_t)acc * k.mult + base;
+    int32_t d = (int32_t)__funnelshift_r((uint32_t)t, (uint32_t)(t >> 32), k.shift);
     d = d < k.limit ? k.below : d;
     const float x = __int_as_float(d);
     const float f = __fadd_rn(x, __fadd_rn(__fmaf_rd(x, 0.5f, 6291456.f), -__fmaf_rd(x, 0.0625f, 11796480.f)));
@@ -659,7 +669,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     const RrsK rk = rrs_k(a.qk_shift);
     const FastExp fx = fast_exp(a);
     const FinishK fk{rrs_k(a.rsqrt_offset), rrs_k(a.av_shift), a.av_mult};
-    const bool fast_ok = a.frac_bits >= 7 && a.frac_bits <= 14 && a.qk_shift >= 2 && a.qk_shift <= 30;
+    const bool fast_ok = a.frac_bits >= 7 && a.frac_bits <= 14 && a.qk_shift >= 1 && a.qk_shift <= 9;
     const int cut = min(22795, 8 << min(max(a.frac_bits, 7), 14));
     auto requant = [&](int32_t acc) { return clampi(rrs_apply(wmul(acc, a.qk_mult), rk), -32768, 32767); };
     auto meet = [&] {
@@ -671,12 +681,29 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     // rows need another order than 64-byte ones so that neither the K nor the V
     // fragments meet bank conflicts
     auto order = [](int k) { return D == 64 ? k : 8 * (k >> 3) + 4 * (k & 1) + 2 * ((k >> 1) & 1) + ((k >> 2) & 1); };
-    const int krow0 = order(4 * (g >> 1) + (g & 1)), krow1 = order(4 * (g >> 1) + 2 + (g & 1));
+    // lane offsets in a tile: its K piece of score tile jj and 64-byte half h, its V
+    // row of piece 0 (piece c: the same with bits 4.. flipped by c)
+    uint32_t koff[2][D / 64];
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+            const int row = order(4 * (g >> 1) + 2 * jj + (g & 1));
+            koff[jj][h] = row * D + swz<D>(row, 4 * h + t) * 16;
+        }
     const int vrow = (lane & 16) + order(lane & 15);
+    const uint32_t voff = vrow * D + swz<D>(vrow, 0) * 16;
+
+    bool holes = false;  // keys of this block without a page
+    for (int j = (((first * kTile) >> a.page_log2) + lane) << a.page_log2; j < min((first + mine) * kTile, r.keys);
+         j += 32 << a.page_log2)
+        holes |= !has_page(a, r, j);
+    const int all_see = __any_sync(0xffffffffu, holes) ? 0 : min(r.ctx, r.keys);  // keys below are seen by every row
 
     uint32_t n = 0;  // tiles of this set's slots seen so far
     auto slot = [&](uint32_t n) { return (kg << lsg) + (n & (SG - 1)); };
-    auto tile_at = [&](uint32_t n) { return smem + slot(n) * F::kBytes; };
+    const uint32_t ring = smem_u32(smem);
+    auto tile_at = [&](uint32_t n) { return ring + slot(n) * F::kBytes; };
     auto arrived = [&](uint32_t n) { slab_wait(&full[slot(n)], (n >> lsg) & 1); };
     auto release = [&](uint32_t n) {
         __syncwarp();
@@ -701,9 +728,9 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
 
         // which keys j0 .. j0+31 the rows ra and rb see; true when all of them by all
         auto seen = [&](int j0, uint32_t &wa, uint32_t &wb) {
-            const uint32_t there = __ballot_sync(0xffffffffu, has_page(a, r, j0 + lane));
-            wa = wb = there;
-            if (j0 + 32 <= r.ctx) return there == 0xffffffffu;
+            if (j0 + 32 <= all_see) return true;
+            wa = wb = __ballot_sync(0xffffffffu, has_page(a, r, j0 + lane));
+            if (j0 + 32 <= r.ctx) return false;
             const int u0 = j0 - r.ctx;  // place of the first key among the new tokens
             auto word = [&](int n) -> uint32_t {
                 if (a.words == 0) return n < u0 ? 0u : (n - u0 >= 31 ? 0xffffffffu : (2u << (n - u0)) - 1);
@@ -717,15 +744,14 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             return false;
         };
         // raw scores of 32 keys: c[2 * half + jj], columns order(4t + 2jj + e) + 16 * half
-        auto raw = [&](int32_t (&c)[4][4], const uint8_t *ks) {
+        auto raw = [&](int32_t (&c)[4][4], uint32_t ks) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int row = 16 * (j >> 1) + ((j & 1) ? krow1 : krow0);
-                c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0;
 #pragma unroll
                 for (int h = 0; h < D / 64; ++h) {
-                    const int4 k = *reinterpret_cast<const int4 *>(ks + row * D + swz<D>(row, 4 * h + t) * 16);
-                    mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
+                    const int4 k = lds_v4(ks + 16 * (j >> 1) * D + koff[j & 1][h]);
+                    if (h == 0) mma_s8_first(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
+                    else mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
                     mma_s8(c[j], q0[h].z, q1[h].z, q0[h].w, q1[h].w, k.z, k.w);
                 }
             }
@@ -776,11 +802,15 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
         }
         const int32_t xa = (m0 == INT32_MIN ? -32768 : requant(m0)) + 1, xb = (m1 == INT32_MIN ? -32768 : requant(m1)) + 1;
         auto inside = [&](int32_t xm) { return xm <= 32767 && xm - cut >= -32768; };
+        const int64_t base_a = fast_base(xa, fx), base_b = fast_base(xb, fx);
         const bool fast = __all_sync(0xffffffffu, fast_ok && (ra >= rows || inside(xa)) && (rb >= rows || inside(xb)));
 
-        int32_t o[D / 8][4];
+        // (P.V)^T: channels 16i + g (and + 8) of rows 2t, 2t+1 of either 8 rows
+        int32_t o[D / 16][2][4];
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0;
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[i][e >> 2][e & 3] = 0;
         uint32_t sum0 = 0, sum1 = 0;
         for (int i = kg; i < mine; i += KG, n += 2) {
             uint32_t p[kTile / 32][4];
@@ -793,7 +823,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) c[j][e] = (int32_t)fast_prob(c[j][e], kBias - (e < 2 ? xa : xb), fx);
+                        for (int e = 0; e < 4; ++e) c[j][e] = (int32_t)fast_prob(c[j][e], e < 2 ? base_a : base_b, fx);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -826,16 +856,15 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             }
             release(n);
             arrived(n + 1);
-            const uint8_t *vs = tile_at(n + 1);
+            const uint32_t vs = tile_at(n + 1) + voff;
 #pragma unroll
             for (int c = 0; c < D / 16; ++c)
 #pragma unroll
                 for (int h32 = 0; h32 < kTile / 32; ++h32) {
-                    const int row = 32 * h32 + vrow;
                     uint32_t v[4];
-                    ldsm_trans_b8(v, vs + row * D + swz<D>(row, c) * 16);
-                    mma_u8s8(o[2 * c], p[h32][0], p[h32][1], p[h32][2], p[h32][3], v[0], v[2]);
-                    mma_u8s8(o[2 * c + 1], p[h32][0], p[h32][1], p[h32][2], p[h32][3], v[1], v[3]);
+                    ldsm_trans_b8(v, (vs ^ (16 * c)) + 32 * h32 * D);
+                    mma_s8u8(o[c][0], v[0], v[1], v[2], v[3], p[h32][0], p[h32][2]);
+                    mma_s8u8(o[c][1], v[0], v[1], v[2], v[3], p[h32][1], p[h32][3]);
                 }
             release(n + 1);
         }
@@ -849,12 +878,14 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             else *d = v;
         };
         if (t == 0) give(&s_sum[16 * rt + g], (int32_t)sum0), give(&s_sum[16 * rt + g + 8], (int32_t)sum1);
-        int32_t *d0 = s_o + (16 * rt + g) * OLD + 2 * t;
+        int32_t *d0 = s_o + (16 * rt + 2 * t) * OLD + g;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-            give(d0 + 8 * c, o[c][0]), give(d0 + 8 * c + 1, o[c][1]);
-            give(d0 + 8 * OLD + 8 * c, o[c][2]), give(d0 + 8 * OLD + 8 * c + 1, o[c][3]);
-        }
+        for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                int32_t *d = d0 + 8 * e * OLD + 16 * c;
+                give(d, o[c][e][0]), give(d + OLD, o[c][e][1]), give(d + 8, o[c][e][2]), give(d + OLD + 8, o[c][e][3]);
+            }
         meet();
         auto total = [&](int32_t *p, int i) {
             if (ranks == 1) return p[i];
