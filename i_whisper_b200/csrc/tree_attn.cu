@@ -26,18 +26,18 @@ struct Slab {
 // the same rows, k 16+4t..; b0/b1: column g, k 4t.. / 16+4t..; c0,c1/c2,c3:
 // rows g/g+8, columns 2t, 2t+1.
 IW_DEV void mma_s8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 IW_DEV void mma_s8u8(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // c = a * b, signed.
 IW_DEV void mma_s8_first(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
                  : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
@@ -47,12 +47,11 @@ IW_DEV void mma_s8_first(int32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
 IW_DEV void ldsm_trans_b8(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(at)
-                 : "memory");
+                 : "r"(at));
 }
 IW_DEV int4 lds_v4(uint32_t at) {
     int4 v;
-    asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    asm volatile("ld.shared.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
 }
 
@@ -117,6 +116,49 @@ IW_DEV int32_t finish(const FinishK &k, int32_t acc, int32_t inv) {
     return clampi(rrs_apply(wmul(v, k.av_mult), k.out), -127, 127);
 }
 
+// Maximum or sum over the cluster's blocks of one value or four of their shared
+// memory, four blocks' loads in flight at a time (a load from another block
+// takes hundreds of cycles). A rank count of 1, 2, 4 or 8.
+IW_DEV int32_t cluster_max(cooperative_groups::cluster_group cl, int32_t *p, int ranks) {
+    int32_t m = INT32_MIN;
+    for (int k0 = 0; k0 < ranks; k0 += 4) {
+        int32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = *cl.map_shared_rank(p, (k0 + k) & (ranks - 1));
+        m = max(max(m, max(v[0], v[1])), max(v[2], v[3]));
+    }
+    return m;
+}
+IW_DEV int32_t cluster_sum(cooperative_groups::cluster_group cl, int32_t *p, int ranks) {
+    int32_t sum = 0;
+    for (int k0 = 0; k0 < ranks; k0 += 4) {
+        int32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = *cl.map_shared_rank(p, (k0 + k) & (ranks - 1));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum += k0 + k < ranks ? v[k] : 0;
+    }
+    return sum;
+}
+IW_DEV int4 cluster_sum4(cooperative_groups::cluster_group cl, int32_t *p, int ranks) {
+    int4 sum = make_int4(0, 0, 0, 0);
+    for (int k0 = 0; k0 < ranks; k0 += 4) {
+        int4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            v[k] = *reinterpret_cast<const int4 *>(cl.map_shared_rank(p, (k0 + k) & (ranks - 1)));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k0 + k < ranks) sum.x += v[k].x, sum.y += v[k].y, sum.z += v[k].z, sum.w += v[k].w;
+    }
+    return sum;
+}
+// Four channels normalised, as bytes.
+IW_DEV uint32_t finish4(const FinishK &k, int4 v, int32_t inv) {
+    return (uint32_t)(finish(k, v.x, inv) & 255) | (uint32_t)(finish(k, v.y, inv) & 255) << 8 |
+           (uint32_t)(finish(k, v.z, inv) & 255) << 16 | (uint32_t)(finish(k, v.w, inv) & 255) << 24;
+}
+
 // Rows from starts[B] on are padding: the blocks of the last request zero
 // them, each its own heads.
 IW_DEV void zero_padding(const TreeAttnArgs &a, int kvh, int rank, int ranks) {
@@ -149,7 +191,7 @@ IW_DEV void load_boxes(const TreeAttnArgs &a, const CUtensorMap *map, int kvh, i
         tma_load_4d(map, bar, dst + lane * box * D, 0, (j0 + lane * box) & ((1 << a.page_log2) - 1), kvh, page);
 }
 template <int D, int BYTES>
-IW_DEV void load_rows(const TreeAttnArgs &a, const Request &r, const int8_t *head, int j0, uint8_t *dst, uint64_t *bar) {
+IW_DEV void load_rows(const TreeAttnArgs &a, const Request &r, const int8_t *head, int j0, uint8_t *dst) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int e = 0; e < BYTES / 512; ++e) {
@@ -157,7 +199,6 @@ IW_DEV void load_rows(const TreeAttnArgs &a, const Request &r, const int8_t *hea
         if (has_page(a, r, j))
             cp_async16(dst + row * D + swz<D>(row, c) * 16, head + row_at(a, r.table[j >> a.page_log2], j) + 16 * c);
     }
-    mbar_arrive_cp_async(bar);
 }
 // Bounded wait of a warp for a slab. A wait that gives up sets the device
 // status word, and this warp's later waits then give up after a millisecond each,
@@ -284,7 +325,8 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
                 load_boxes<D>(a, v ? &tmap_v : &tmap_k, kvh, j0, box, page, lane < per && page >= 0, ring + slot * 4096,
                               &bars[slot]);
             } else {
-                load_rows<D, 4096>(a, r, v ? vbase : kbase, j0, ring + slot * 4096, &bars[slot]);
+                load_rows<D, 4096>(a, r, v ? vbase : kbase, j0, ring + slot * 4096);
+                mbar_arrive_cp_async(&bars[slot]);
             }
         };
         auto arrived = [&](int it) -> const uint8_t * {
@@ -412,8 +454,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
             } else {
                 cg::cluster_group cl = cg::this_cluster();
                 cl.sync();
-                xm = INT32_MIN;
-                for (int k = 0; k < ranks; ++k) xm = max(xm, cl.map_shared_rank(s_max, k)[lane & (NR - 1)]);
+                xm = cluster_max(cl, s_max + (lane & (NR - 1)), ranks);
             }
         }
         xm = (xm == INT32_MIN ? -32768 : requant(xm)) + 1;
@@ -496,33 +537,28 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
                 for (int c = 0; c < D / 16; ++c) give(d + OLD + 16 * c, o[c][1]), give(d + OLD + 16 * c + 8, o[c][3]);
             }
         }
-        auto write = [&](auto total) {  // two channels per thread, dealt out over the cluster
-            int32_t inv = 0;            // row = lane
-            if (lane < nr) inv = fisr(total(s_sum, lane), a.rsqrt_offset);
+        auto write = [&](auto total, auto total4) {  // four channels per thread, dealt out over the cluster
+            int32_t inv = 0;                         // row = lane
+            if (lane < nr) inv = fisr(total(s_sum + lane), a.rsqrt_offset);
 #pragma unroll 1
-            for (int i0 = (rank * W + warp) * 32; i0 < nr * (D / 2); i0 += ranks * W * 32) {
-                const int i = i0 + lane, k = i0 / (D / 2), d = (i % (D / 2)) * 2, row = row0 + k, n = token(row);
-                const int32_t v = __shfl_sync(0xffffffffu, inv, k);
-                char2 w;
-                w.x = (signed char)finish(fk, total(s_o, k * OLD + d), v);
-                w.y = (signed char)finish(fk, total(s_o, k * OLD + d + 1), v);
-                *reinterpret_cast<char2 *>(a.y + (int64_t)(r.first + n) * a.ldy + (int64_t)(kvh * G + row - n * G) * D + d) = w;
+            for (int i0 = (rank * W + warp) * 32; i0 < nr * (D / 4); i0 += ranks * W * 32) {
+                const int i = i0 + lane, k = i / (D / 4), d = (i % (D / 4)) * 4, row = row0 + k, n = token(row);
+                const int32_t v = __shfl_sync(0xffffffffu, inv, k & 31);
+                if (k < nr)
+                    *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + n) * a.ldy + (int64_t)(kvh * G + row - n * G) * D +
+                                                  d) = finish4(fk, total4(s_o + k * OLD + d), v);
             }
         };
         if (ranks == 1) {
             if (W > 1) __syncthreads();
             else __syncwarp();
-            write([&](int32_t *p, int i) { return p[i]; });
+            write([](int32_t *p) { return *p; }, [](int32_t *p) { return *reinterpret_cast<const int4 *>(p); });
             if (W > 1) __syncthreads();
             else __syncwarp();
         } else {
             cg::cluster_group cl = cg::this_cluster();
             cl.sync();
-            write([&](int32_t *p, int i) {
-                uint32_t v = 0;
-                for (int k = 0; k < ranks; ++k) v += (uint32_t)cl.map_shared_rank(p, k)[i];
-                return (int32_t)v;
-            });
+            write([&](int32_t *p) { return cluster_sum(cl, p, ranks); }, [&](int32_t *p) { return cluster_sum4(cl, p, ranks); });
             cl.sync();  // no block's sums go away or are cleared while another reads them
         }
     }
@@ -532,7 +568,7 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
 // Many rows per key head (trees, prompts, shared key heads): bound by the
 // arithmetic of the integer softmax and the score products. A block, or a
 // cluster of them that splits the keys, serves one (request, key head); four
-// warps compute, a fifth feeds a ring of 64-key K and V tiles by TMA (a full
+// warps compute, a fifth feeds a ring of 4 KB K and V tiles by TMA (a full
 // and an empty barrier per tile). A warp holds 16 rows: scores by mma.sync, the
 // keys of a tile in such an order that a thread's four probabilities are four
 // consecutive operand bytes of P.V, which therefore never leave registers; V
@@ -544,12 +580,12 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
 // tensor memory, from where the softmax has to fetch them, and it wants 128
 // rows, which trees of 64 tokens on one head do not have.
 // ---------------------------------------------------------------------------
-constexpr int kManyWarps = 4, kTile = 64;
+constexpr int kManyWarps = 4;
 
 template <int D>
 struct Many {
     static constexpr int kStages = 8;
-    static constexpr int kBytes = kTile * D;
+    static constexpr int kBytes = 64 * D;  // 64 keys of K, or 32 of K and the same of V
     static constexpr int kOutLd = D + 4;
     static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * (kOutLd + 2) * 4; }
 };
@@ -605,7 +641,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_align1024(smem_raw);
     using F = Many<D>;
-    constexpr int S = F::kStages, OLD = F::kOutLd;
+    constexpr int S = F::kStages, OLD = F::kOutLd, kTile = 64;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * F::kBytes), *empty = full + S;
     int32_t *s_o = reinterpret_cast<int32_t *>(empty + S), *s_sum = s_o + 64 * OLD, *s_max = s_sum + 64;
@@ -619,8 +655,8 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     const int rows = r.fresh * G;
     if (rows == 0) return;
     // RT groups of 16 rows side by side, KG sets of warps that share out the tiles:
-    // set i takes tiles i, i + KG, ... through SG slots of the ring that are its own (a
-    // set has to see every phase of the barriers it waits on)
+    // set i takes tiles of 64 keys i, i + KG, ... through SG slots of the ring that
+    // are its own (a set has to see every phase of the barriers it waits on)
     const int lrt = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2), lkg = 2 - lrt, lsg = 3 - lkg;
     static_assert(kManyWarps == 4 && S == 8, "powers of two above");
     const int RT = 1 << lrt, KG = 1 << lkg, SG = 1 << lsg;
@@ -637,29 +673,55 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
 
     if (warp == kManyWarps) {  // the feeder: K tiles, then K and V tiles in turn, for every block of rows
         const int8_t *kbase = a.k + kvh * a.head_stride, *vbase = a.v + kvh * a.head_stride;
-        const int box = min(1 << a.page_log2, kTile);
+        // lane i holds the page of box i of a window of 32 boxes (the table's latency
+        // would otherwise be paid for every slot); boxes of at most 32 rows
+        const int box = min(1 << a.page_log2, 32), per = 32 / box;
+        int32_t pages = -1;
+        auto window = [&](int i) {
+            const int j = first * kTile + i * 32 + lane * box;
+            pages = j < min((first + mine) * kTile, r.keys) ? r.table[j >> a.page_log2] : -1;
+            if ((uint32_t)pages >= a.n_pages) pages = -1;
+        };
+        if (TMA) window(0);
         uint32_t done = 0;  // blocks of rows fed
-        auto put = [&](bool pass2, bool v, int i) {
-            const uint32_t set = i & (KG - 1), at = i >> lkg, count = (mine - set + KG - 1) >> lkg;
-            const uint32_t n = 3 * count * done + (pass2 ? count + 2 * at + v : at), slot = (set << lsg) + (n & (SG - 1));
+        // slot `at` of a set's in this block of rows, filled with the 32 keys of half
+        // tile i and, of the first pass, the next 32, of the second, their V
+        auto put = [&](int set, int at, int i, bool pass2) {
+            const uint32_t count = (mine - set + KG - 1) >> lkg, n = 3 * count * done + (pass2 ? count : 0) + at;
+            const uint32_t slot = (set << lsg) + (n & (SG - 1));
             if (n >= SG) slab_wait(&empty[slot], ((n >> lsg) - 1) & 1);
-            const int j0 = (first + i) * kTile;
             uint8_t *dst = smem + slot * F::kBytes;
+            const int j0 = first * kTile + i * 32;
             if (TMA) {
-                const int j = j0 + lane * box;
-                const int32_t page = lane * box < kTile && j < r.keys ? r.table[j >> a.page_log2] : -1;
-                load_boxes<D>(a, v ? &tmap_v : &tmap_k, kvh, j0, box, page, (uint32_t)page < a.n_pages, dst, &full[slot]);
+                const int w = (i * per) & 31;
+                if (w == 0 && mine * 2 * per > 32) window(i);
+                const int32_t page = __shfl_sync(0xffffffffu, pages, pass2 ? w + (lane & (per - 1)) : w + lane);
+                const bool ok = lane < 2 * per && page >= 0;
+                const uint32_t n_box = __popc(__ballot_sync(0xffffffffu, ok));
+                if (lane == 0) mbar_arrive_expect_tx(&full[slot], n_box * box * D);
+                __syncwarp();
+                const bool v = pass2 && lane >= per;
+                const int j = j0 + (v ? lane - per : lane) * box;
+                if (ok)
+                    tma_load_4d(v ? &tmap_v : &tmap_k, &full[slot], dst + lane * box * D, 0, j & ((1 << a.page_log2) - 1), kvh,
+                                page);
             } else {
-                load_rows<D, F::kBytes>(a, r, v ? vbase : kbase, j0, dst, &full[slot]);
+                load_rows<D, 32 * D>(a, r, kbase, j0, dst);
+                load_rows<D, 32 * D>(a, r, pass2 ? vbase : kbase, pass2 ? j0 : j0 + 32, dst + 32 * D);
+                mbar_arrive_cp_async(&full[slot]);
             }
         };
+        auto put2 = [&](int i) {  // half tile i of the second pass
+            const int tile = i >> 1;
+            put(tile & (KG - 1), 2 * (tile >> lkg) + (i & 1), i, true);
+        };
         for (int row0 = 0; row0 < rows; row0 += 16 * RT, ++done) {
-            for (int i = 0; i < mine; ++i) put(false, false, i);
-            // a ring of the second pass's tiles goes out before the blocks meet
+            for (int i = 0; i < mine; ++i) put(i & (KG - 1), i >> lkg, 2 * i, false);
+            // a ring of the second pass's slots goes out before the blocks meet
             const int ahead = min(S, 2 * mine);
-            for (int i = 0; i < ahead; ++i) put(true, i & 1, i >> 1);
+            for (int i = 0; i < ahead; ++i) put2(i);
             if (ranks > 1) cl.sync();
-            for (int i = ahead; i < 2 * mine; ++i) put(true, i & 1, i >> 1);
+            for (int i = ahead; i < 2 * mine; ++i) put2(i);
             if (ranks > 1) cl.sync(), cl.sync();
         }
         return;
@@ -723,7 +785,10 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 q1[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + tb) * a.ldq +
                                                         (int64_t)(kvh * G + rb - tb * G) * a.q_hs + 64 * c + 16 * t);
         }
-        for (int i = tid; i < 64 * (OLD + 2); i += 32 * kManyWarps) s_o[i] = i < 64 * OLD + 64 ? 0 : INT32_MIN;
+        if (KG > 1)
+            for (int i = tid; i < 16 * RT * OLD / 4; i += 32 * kManyWarps)
+                reinterpret_cast<int4 *>(s_o)[i] = make_int4(0, 0, 0, 0);
+        if (tid < 64) s_sum[tid] = 0, s_max[tid] = INT32_MIN;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");
 
         // which keys j0 .. j0+31 the rows ra and rb see; true when all of them by all
@@ -746,14 +811,17 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
         // raw scores of 32 keys: c[2 * half + jj], columns order(4t + 2jj + e) + 16 * half
         auto raw = [&](int32_t (&c)[4][4], uint32_t ks) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int h = 0; h < D / 64; ++h) {
+                int4 k[4];
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h) {
-                    const int4 k = lds_v4(ks + 16 * (j >> 1) * D + koff[j & 1][h]);
-                    if (h == 0) mma_s8_first(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
-                    else mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k.x, k.y);
-                    mma_s8(c[j], q0[h].z, q1[h].z, q0[h].w, q1[h].w, k.z, k.w);
+                for (int j = 0; j < 4; ++j) k[j] = lds_v4(ks + 16 * (j >> 1) * D + koff[j & 1][h]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (h == 0) mma_s8_first(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k[j].x, k[j].y);
+                    else mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k[j].x, k[j].y);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_s8(c[j], q0[h].z, q1[h].z, q0[h].w, q1[h].w, k[j].z, k[j].w);
             }
         };
         auto bit = [&](int j, int e) { return 16 * (j >> 1) + order(4 * t + 2 * (j & 1) + e); };
@@ -762,7 +830,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
         for (int i = kg; i < mine; i += KG, ++n) {
             arrived(n);
 #pragma unroll
-            for (int h32 = 0; h32 < kTile / 32; ++h32) {
+            for (int h32 = 0; h32 < 2; ++h32) {
                 int32_t c[4][4];
                 raw(c, tile_at(n) + h32 * 32 * D);
                 uint32_t wa, wb;
@@ -794,11 +862,8 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             m0 = s_max[16 * rt + g];
             m1 = s_max[16 * rt + g + 8];
         } else {
-            for (int k = 0; k < ranks; ++k) {
-                const int32_t *o = cl.map_shared_rank(s_max, k);
-                m0 = max(m0, o[16 * rt + g]);
-                m1 = max(m1, o[16 * rt + g + 8]);
-            }
+            m0 = cluster_max(cl, s_max + 16 * rt + g, ranks);
+            m1 = cluster_max(cl, s_max + 16 * rt + g + 8, ranks);
         }
         const int32_t xa = (m0 == INT32_MIN ? -32768 : requant(m0)) + 1, xb = (m1 == INT32_MIN ? -32768 : requant(m1)) + 1;
         auto inside = [&](int32_t xm) { return xm <= 32767 && xm - cut >= -32768; };
@@ -812,13 +877,13 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[i][e >> 2][e & 3] = 0;
         uint32_t sum0 = 0, sum1 = 0;
-        for (int i = kg; i < mine; i += KG, n += 2) {
-            uint32_t p[kTile / 32][4];
+        for (int i = 0; i < 2 * ((mine - kg + KG - 1) >> lkg); ++i, ++n) {
+            const int j0 = (first + kg + (i >> 1) * KG) * kTile + 32 * (i & 1);
+            uint32_t p[4];
             arrived(n);
-#pragma unroll
-            for (int h32 = 0; h32 < kTile / 32; ++h32) {
+            {
                 int32_t c[4][4];
-                raw(c, tile_at(n) + h32 * 32 * D);
+                raw(c, tile_at(n));
                 if (fast) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -834,39 +899,34 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 auto pack = [](int32_t x, int32_t y, int32_t z, int32_t w) {
                     return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
                 };
-                uint32_t (&a4)[4] = p[h32];
-                a4[0] = pack(c[0][0], c[0][1], c[1][0], c[1][1]);
-                a4[1] = pack(c[0][2], c[0][3], c[1][2], c[1][3]);
-                a4[2] = pack(c[2][0], c[2][1], c[3][0], c[3][1]);
-                a4[3] = pack(c[2][2], c[2][3], c[3][2], c[3][3]);
-                uint32_t wa, wb;
-                if (!seen((first + i) * kTile + 32 * h32, wa, wb)) {
+                p[0] = pack(c[0][0], c[0][1], c[1][0], c[1][1]);
+                p[1] = pack(c[0][2], c[0][3], c[1][2], c[1][3]);
+                p[2] = pack(c[2][0], c[2][1], c[3][0], c[3][1]);
+                p[3] = pack(c[2][2], c[2][3], c[3][2], c[3][3]);
+            }
+            uint32_t wa, wb;
+            if (!seen(j0, wa, wb)) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t w = (x & 1) ? wb : wa;
-                        uint32_t keep = 0;
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t w = (x & 1) ? wb : wa;
+                    uint32_t keep = 0;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if ((w >> (16 * (x >> 1) + order(4 * t + e))) & 1) keep |= 0xffu << (8 * e);
-                        a4[x] &= keep;
-                    }
+                    for (int e = 0; e < 4; ++e)
+                        if ((w >> (16 * (x >> 1) + order(4 * t + e))) & 1) keep |= 0xffu << (8 * e);
+                    p[x] &= keep;
                 }
-                sum0 = __dp4a(a4[0], 0x01010101u, __dp4a(a4[2], 0x01010101u, sum0));
-                sum1 = __dp4a(a4[1], 0x01010101u, __dp4a(a4[3], 0x01010101u, sum1));
+            }
+            sum0 = __dp4a(p[0], 0x01010101u, __dp4a(p[2], 0x01010101u, sum0));
+            sum1 = __dp4a(p[1], 0x01010101u, __dp4a(p[3], 0x01010101u, sum1));
+            const uint32_t vs = tile_at(n) + 32 * D + voff;
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {
+                uint32_t v[4];
+                ldsm_trans_b8(v, vs ^ (16 * c));
+                mma_s8u8(o[c][0], v[0], v[1], v[2], v[3], p[0], p[2]);
+                mma_s8u8(o[c][1], v[0], v[1], v[2], v[3], p[1], p[3]);
             }
             release(n);
-            arrived(n + 1);
-            const uint32_t vs = tile_at(n + 1) + voff;
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c)
-#pragma unroll
-                for (int h32 = 0; h32 < kTile / 32; ++h32) {
-                    uint32_t v[4];
-                    ldsm_trans_b8(v, (vs ^ (16 * c)) + 32 * h32 * D);
-                    mma_s8u8(o[c][0], v[0], v[1], v[2], v[3], p[h32][0], p[h32][2]);
-                    mma_s8u8(o[c][1], v[0], v[1], v[2], v[3], p[h32][1], p[h32][3]);
-                }
-            release(n + 1);
         }
         // sums over the warps that shared the tiles, then over the cluster
         sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
@@ -887,23 +947,23 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 give(d, o[c][e][0]), give(d + OLD, o[c][e][1]), give(d + 8, o[c][e][2]), give(d + OLD + 8, o[c][e][3]);
             }
         meet();
-        auto total = [&](int32_t *p, int i) {
-            if (ranks == 1) return p[i];
-            uint32_t v = 0;
-            for (int k = 0; k < ranks; ++k) v += (uint32_t)cl.map_shared_rank(p, k)[i];
-            return (int32_t)v;
-        };
-        // one row per warp and step, two channels per lane
-        for (int k = rank * kManyWarps + warp; k < min(16 * RT, rows - row0); k += ranks * kManyWarps) {
-            const int row = row0 + k, tok = row / G;
-            const int32_t inv = fisr(total(s_sum, k), a.rsqrt_offset);
-            int8_t *out = a.y + (int64_t)(r.first + tok) * a.ldy + (int64_t)(kvh * G + row - tok * G) * D;
-#pragma unroll
-            for (int d = 2 * lane; d < D; d += 64) {
-                char2 w;
-                w.x = (signed char)finish(fk, total(s_o, k * OLD + d), inv);
-                w.y = (signed char)finish(fk, total(s_o, k * OLD + d + 1), inv);
-                *reinterpret_cast<char2 *>(out + d) = w;
+        // rows dealt out over the cluster and the warps, four channels per lane
+        constexpr int kAtOnce = 128 / D;  // rows per step of a warp
+        const int nr = min(16 * RT, rows - row0), first_k = (rank * kManyWarps + warp) * kAtOnce, step = ranks * kManyWarps * kAtOnce;
+        int32_t inv = 0;  // of the warp's row first_k + (lane / kAtOnce) * step + lane % kAtOnce
+        {
+            const int k = first_k + lane / kAtOnce * step + lane % kAtOnce;
+            if (k < nr) inv = fisr(ranks == 1 ? s_sum[k] : cluster_sum(cl, s_sum + k, ranks), a.rsqrt_offset);
+        }
+#pragma unroll 1
+        for (int k0 = first_k, i = 0; k0 < nr; k0 += step, i += kAtOnce) {
+            const int k = k0 + lane / (D / 4), d = lane % (D / 4) * 4, row = row0 + k, tok = G == 1 ? row : row / G;
+            const int32_t v = __shfl_sync(0xffffffffu, inv, i + lane / (D / 4));
+            if (k < nr) {
+                int32_t *p = s_o + k * OLD + d;
+                const int4 x = ranks == 1 ? *reinterpret_cast<const int4 *>(p) : cluster_sum4(cl, p, ranks);
+                *reinterpret_cast<uint32_t *>(a.y + (int64_t)(r.first + tok) * a.ldy + (int64_t)(kvh * G + row - tok * G) * D +
+                                              d) = finish4(fk, x, v);
             }
         }
         meet();  // no block's sums go away or are cleared while another reads them
@@ -934,10 +994,10 @@ static cudaError_t launch_cluster(void (*kernel)(KArgs...), int ranks, dim3 grid
 struct CacheMaps {
     CUtensorMap k, v;
 };
-static cudaError_t cache_maps(const TreeAttnArgs &a, int rows, CacheMaps &m) {
+static cudaError_t cache_maps(const TreeAttnArgs &a, int box_rows, CacheMaps &m) {
     const uint64_t sizes[4] = {(uint64_t)a.D, 1ull << a.page_log2, (uint64_t)a.Hkv, a.n_pages};
     const uint64_t strides[3] = {a.row_stride, (uint64_t)a.head_stride, a.page_stride};
-    const uint32_t box[4] = {(uint32_t)a.D, std::min(1u << a.page_log2, (unsigned)rows), 1, 1};
+    const uint32_t box[4] = {(uint32_t)a.D, std::min(1u << a.page_log2, (unsigned)box_rows), 1, 1};
     const CUtensorMapSwizzle swz = a.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
     cudaError_t e = make_tmap_4d_u8(&m.k, a.k, sizes, strides, box, swz);
     return e == cudaSuccess ? make_tmap_4d_u8(&m.v, a.v, sizes, strides, box, swz) : e;
@@ -1016,7 +1076,7 @@ static cudaError_t attention(const TreeAttnArgs &a, cudaStream_t st) {
     const bool many = mean_rows > kFewRows;
     CacheMaps m = {};
     if (tma)
-        if (cudaError_t e = cache_maps(a, many ? kTile : Slab<D>::kKeys, m); e != cudaSuccess) return e;
+        if (cudaError_t e = cache_maps(a, many ? 32 : Slab<D>::kKeys, m); e != cudaSuccess) return e;
     if (!many) return few_rows<D>(a, m, tma, mean_rows, st);
     return tma ? many_rows<D, true>(a, m, st) : many_rows<D, false>(a, m, st);
 }
