@@ -774,17 +774,22 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     for (int row0 = 0; row0 < rows; row0 += 16 * RT) {
         const int ra = row0 + 16 * rt + g, rb = ra + 8;  // this lane's rows
         const int ta = G == 1 ? ra : ra / G, tb = G == 1 ? rb : rb / G;
-        int4 q0[D / 64], q1[D / 64];
+        // the 16-row operand of step s of half c: bytes 16t + 8s.. and 16t + 8s + 4.. of
+        // rows ra, rb. Loaded word by word: out of 16-byte loads the compiler moved the
+        // registers into operand order again for every product
+        uint32_t q[D / 64][2][4];
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            q0[c] = q1[c] = make_int4(0, 0, 0, 0);
-            if (ra < rows)
-                q0[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + ta) * a.ldq +
-                                                        (int64_t)(kvh * G + ra - ta * G) * a.q_hs + 64 * c + 16 * t);
-            if (rb < rows)
-                q1[c] = *reinterpret_cast<const int4 *>(a.q + (int64_t)(r.first + tb) * a.ldq +
-                                                        (int64_t)(kvh * G + rb - tb * G) * a.q_hs + 64 * c + 16 * t);
-        }
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                auto word = [&](int row, int tok) -> uint32_t {
+                    if (row >= rows) return 0;
+                    return *reinterpret_cast<const uint32_t *>(a.q + (int64_t)(r.first + tok) * a.ldq +
+                                                               (int64_t)(kvh * G + row - tok * G) * a.q_hs + 64 * c + 16 * t + 4 * x);
+                };
+                q[c][x >> 1][2 * (x & 1)] = word(ra, ta);
+                q[c][x >> 1][2 * (x & 1) + 1] = word(rb, tb);
+            }
         if (KG > 1)
             for (int i = tid; i < 16 * RT * OLD / 4; i += 32 * kManyWarps)
                 reinterpret_cast<int4 *>(s_o)[i] = make_int4(0, 0, 0, 0);
@@ -817,11 +822,12 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 for (int j = 0; j < 4; ++j) k[j] = lds_v4(ks + 16 * (j >> 1) * D + koff[j & 1][h]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (h == 0) mma_s8_first(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k[j].x, k[j].y);
-                    else mma_s8(c[j], q0[h].x, q1[h].x, q0[h].y, q1[h].y, k[j].x, k[j].y);
+                    uint32_t (&w)[4] = q[h][0];
+                    if (h == 0) mma_s8_first(c[j], w[0], w[1], w[2], w[3], k[j].x, k[j].y);
+                    else mma_s8(c[j], w[0], w[1], w[2], w[3], k[j].x, k[j].y);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma_s8(c[j], q0[h].z, q1[h].z, q0[h].w, q1[h].w, k[j].z, k[j].w);
+                for (int j = 0; j < 4; ++j) mma_s8(c[j], q[h][1][0], q[h][1][1], q[h][1][2], q[h][1][3], k[j].z, k[j].w);
             }
         };
         auto bit = [&](int j, int e) { return 16 * (j >> 1) + order(4 * t + 2 * (j & 1) + e); };
