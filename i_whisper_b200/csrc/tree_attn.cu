@@ -646,20 +646,21 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * F::kBytes), *empty = full + S;
     int32_t *s_o = reinterpret_cast<int32_t *>(empty + S), *s_sum = s_o + 64 * OLD, *s_max = s_sum + 64;
     const int lr = 31 - __clz(ranks);  // a power of two
-    const int rank = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+    const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, b = blockIdx.z, G = a.G;
     if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     pdl_wait();
     pdl_launch();
-    if (b == a.B - 1) zero_padding(a, kvh, rank, ranks);
+    if (b == a.B - 1) zero_padding(a, kvh, blockIdx.x, gridDim.x);
     const Request r = request(a, b);
     const int rows = r.fresh * G;
-    if (rows == 0) return;
     // RT groups of 16 rows side by side, KG sets of warps that share out the tiles:
     // set i takes tiles of 64 keys i, i + KG, ... through SG slots of the ring that
     // are its own (a set has to see every phase of the barriers it waits on)
     const int lrt = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2), lkg = 2 - lrt, lsg = 3 - lkg;
     static_assert(kManyWarps == 4 && S == 8, "powers of two above");
     const int RT = 1 << lrt, KG = 1 << lkg, SG = 1 << lsg;
+    const int first_row = (int)(blockIdx.x >> lr) * 16 * RT, row_step = (int)(gridDim.x >> lr) * 16 * RT;
+    if (first_row >= rows) return;
     if (tid < S) {
         mbar_init(&full[tid], TMA ? 1 : 32);
         mbar_init(&empty[tid], RT);
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             const int tile = i >> 1;
             put(tile & (KG - 1), 2 * (tile >> lkg) + (i & 1), i, true);
         };
-        for (int row0 = 0; row0 < rows; row0 += 16 * RT, ++done) {
+        for (int row0 = first_row; row0 < rows; row0 += row_step, ++done) {
             for (int i = 0; i < mine; ++i) put(i & (KG - 1), i >> lkg, 2 * i, false);
             // a ring of the second pass's slots goes out before the blocks meet
             const int ahead = min(S, 2 * mine);
@@ -771,7 +772,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[slot(n)]);
     };
-    for (int row0 = 0; row0 < rows; row0 += 16 * RT) {
+    for (int row0 = first_row; row0 < rows; row0 += row_step) {
         const int ra = row0 + 16 * rt + g, rb = ra + 8;  // this lane's rows
         const int ta = G == 1 ? ra : ra / G, tb = G == 1 ? rb : rb / G;
         // the 16-row operand of step s of half c: bytes 16t + 8s.. and 16t + 8s + 4.. of
@@ -1059,17 +1060,20 @@ static cudaError_t few_rows(const TreeAttnArgs &a, const CacheMaps &m, bool tma,
 }
 
 template <int D, bool TMA>
-static cudaError_t many_rows(const TreeAttnArgs &a, const CacheMaps &m, cudaStream_t st) {
+static cudaError_t many_rows(const TreeAttnArgs &a, const CacheMaps &m, int64_t mean_rows, cudaStream_t st) {
     const int64_t keys = std::max<int64_t>(1, (int64_t)a.width << a.page_log2), pairs = (int64_t)a.B * a.Hkv;
+    // a row block per 64 rows: as many as the tree mask allows, at most twice the mean's
+    const int64_t most = (a.words ? std::min<int64_t>(a.N, 32 * a.words) : a.N) * a.G;
+    const int row_blocks = (int)std::min<int64_t>(1024, (std::min(most, 2 * mean_rows) + 63) / 64);
     // split the keys while there are fewer than four blocks per SM and a block
     // keeps 256 keys
     int ranks = 1;
-    while (ranks < 8 && pairs * ranks < 4 * num_sms() && keys / ranks > 256) ranks *= 2;
+    while (ranks < 8 && pairs * row_blocks * ranks < 4 * num_sms() && keys / ranks > 256) ranks *= 2;
     const size_t smem = Many<D>::smem();
     static SmemLimit lim;
     cudaError_t e = raise_smem_limit(many_rows_kernel<D, TMA>, smem, lim);
     if (e != cudaSuccess) return e;
-    return launch_cluster(many_rows_kernel<D, TMA>, ranks, dim3(ranks, a.Hkv, a.B), dim3(32 * (kManyWarps + 1)), smem, st,
+    return launch_cluster(many_rows_kernel<D, TMA>, ranks, dim3(ranks * row_blocks, a.Hkv, a.B), dim3(32 * (kManyWarps + 1)), smem, st,
                           m.k, m.v, a, ranks);
 }
 
@@ -1084,7 +1088,7 @@ static cudaError_t attention(const TreeAttnArgs &a, cudaStream_t st) {
     if (tma)
         if (cudaError_t e = cache_maps(a, many ? 32 : Slab<D>::kKeys, m); e != cudaSuccess) return e;
     if (!many) return few_rows<D>(a, m, tma, mean_rows, st);
-    return tma ? many_rows<D, true>(a, m, st) : many_rows<D, false>(a, m, st);
+    return tma ? many_rows<D, true>(a, m, mean_rows, st) : many_rows<D, false>(a, m, mean_rows, st);
 }
 
 }  // namespace tree
