@@ -587,7 +587,9 @@ struct Many {
     static constexpr int kStages = 8;
     static constexpr int kBytes = 64 * D;  // 64 keys of K, or 32 of K and the same of V
     static constexpr int kOutLd = D + 4;
-    static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * (kOutLd + 2) * 4; }
+    // the sums of P.V take the ring's place once the tiles are done with
+    static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * 2 * 4; }
+    static_assert(64 * kOutLd * 4 <= kStages * kBytes, "the sums fit the ring");
 };
 
 // The probability of a score from its raw sum, mostly in the FMA pipe (the ALU
@@ -644,7 +646,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     constexpr int S = F::kStages, OLD = F::kOutLd, kTile = 64;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * F::kBytes), *empty = full + S;
-    int32_t *s_o = reinterpret_cast<int32_t *>(empty + S), *s_sum = s_o + 64 * OLD, *s_max = s_sum + 64;
+    int32_t *s_o = reinterpret_cast<int32_t *>(smem), *s_sum = reinterpret_cast<int32_t *>(empty + S), *s_max = s_sum + 64;
     const int lr = 31 - __clz(ranks);  // a power of two
     const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, b = blockIdx.z, G = a.G;
     if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
@@ -724,6 +726,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             if (ranks > 1) cl.sync();
             for (int i = ahead; i < 2 * mine; ++i) put2(i);
             if (ranks > 1) cl.sync(), cl.sync();
+            __syncthreads();  // the ring is free of sums
         }
         return;
     }
@@ -791,9 +794,6 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 q[c][x >> 1][2 * (x & 1)] = word(ra, ta);
                 q[c][x >> 1][2 * (x & 1) + 1] = word(rb, tb);
             }
-        if (KG > 1)
-            for (int i = tid; i < 16 * RT * OLD / 4; i += 32 * kManyWarps)
-                reinterpret_cast<int4 *>(s_o)[i] = make_int4(0, 0, 0, 0);
         if (tid < 64) s_sum[tid] = 0, s_max[tid] = INT32_MIN;
         asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");
 
@@ -944,6 +944,12 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             if (KG > 1) atomicAdd(d, v);
             else *d = v;
         };
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");  // every tile has been read
+        if (KG > 1) {
+            for (int i = tid; i < 16 * RT * OLD / 4; i += 32 * kManyWarps)
+                reinterpret_cast<int4 *>(s_o)[i] = make_int4(0, 0, 0, 0);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kManyWarps) : "memory");
+        }
         if (t == 0) give(&s_sum[16 * rt + g], (int32_t)sum0), give(&s_sum[16 * rt + g + 8], (int32_t)sum1);
         int32_t *d0 = s_o + (16 * rt + 2 * t) * OLD + g;
 #pragma unroll
@@ -974,6 +980,8 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             }
         }
         meet();  // no block's sums go away or are cleared while another reads them
+        fence_proxy_async_smem();
+        __syncthreads();  // the feeder may fill the ring again
     }
 }
 
