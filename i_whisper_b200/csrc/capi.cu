@@ -817,12 +817,12 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
 
 int iw_token_logprobs(const iw_token_logprobs_desc *d, void *stream) {
     if (!d) return fail(IW_EINVAL, "iw_token_logprobs: null descriptor");
-    if (d->N < 0 || d->N > INT32_MAX || d->V < 1 || d->V > INT32_MAX || d->ld < d->V || d->C < 0)
+    if (d->N < 0 || d->N > INT32_MAX || d->V < 1 || d->V > (1 << 30) || d->ld < d->V || d->C < 0)
         return fail(IW_EINVAL, "iw_token_logprobs: invalid shape");
     if (d->dtype < IW_LOGITS_INT8 || d->dtype > IW_LOGITS_FP32) return fail(IW_EINVAL, "iw_token_logprobs: bad dtype");
     if (d->top < 0 || d->top > IW_LOGPROBS_MAX_TOP || d->top > d->V)
         return fail(IW_EINVAL, "iw_token_logprobs: top must be in [0, min(V, %d)]", IW_LOGPROBS_MAX_TOP);
-    if (!(d->scale > 0.f) || d->scale > 3.0e38f) return fail(IW_EINVAL, "iw_token_logprobs: scale must be positive and finite");
+    if (!(d->scale > 0.f) || d->scale > 1.0e30f) return fail(IW_EINVAL, "iw_token_logprobs: scale must be positive and at most 1e30");
     if (d->N == 0) return IW_OK;
     const int64_t size = d->dtype == IW_LOGITS_INT8 ? 1 : (d->dtype == IW_LOGITS_FP32 ? 4 : 2);
     if (!d->logits || !d->entropy || (d->C && (!d->targets || !d->logprobs)) || (d->top && (!d->top_ids || !d->top_logprobs)))

@@ -2,6 +2,20 @@
 // likely tokens of each row of logits (iw_token_logprobs). With l = scale * x
 // over the tokens that are not suppressed, m = max l and S = sum exp(l - m),
 //   lp(t) = l_t - m - ln S,   H = ln S - sum (l - m) exp(l - m) / S.
+//
+// One block per row reads it once, 16 bytes per thread and load.
+//   Floating types: each thread keeps a running maximum and the sums relative to
+//   it, rescaled when the maximum moves; in units of log 2, so that the
+//   exponential is one instruction. Bound by HBM at 32 bits, by the issue of about
+//   six instructions per element at 16.
+//   int8: there are 256 logits, so the row's histogram says it all: each lane
+//   counts into a column of its own (bank = lane, no conflicts), and the sums
+//   are taken over 256 exact counts. An exponential per element would need more of
+//   its unit than HBM feeds.
+// The most likely tokens: each thread knows its own maximum, so at least
+// `top` elements reach the top-th largest of these; the few elements that do
+// are fetched again (a warp per thread that has some) and ranked among
+// themselves. Rows in which too many do (ties) take a pass per alternative.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -9,110 +23,339 @@
 #include "paged.cuh"
 
 namespace iw {
+namespace lp {
 
-constexpr int kLpThreads = 256;
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kCandidates = 512;
 
-template <typename T>
-IW_DEV float lp_float(T v) { return (float)v; }
-template <>
-IW_DEV float lp_float<__half>(__half v) { return __half2float(v); }
-template <>
-IW_DEV float lp_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+IW_DEV float to_float(int8_t v) { return (float)v; }
+IW_DEV float to_float(float v) { return v; }
+IW_DEV float to_float(__half v) { return __half2float(v); }
+IW_DEV float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// One block per row: maximum, sums, then one pass over the row per
-// alternative. A rank (value, id) is one 64-bit key: the float's bits made
-// to order as an unsigned number, then the id inverted so that the lowest wins.
-IW_DEV uint64_t lp_key(float v, uint32_t id) {
+IW_DEV float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A float's bits made to order as an unsigned number; zeros are equal.
+IW_DEV uint32_t order(float v) {
     const uint32_t b = __float_as_uint(v == 0.f ? 0.f : v);
-    const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return ((uint64_t)o << 32) | (uint32_t)~id;
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
-IW_DEV float lp_key_value(uint64_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
-    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
-}
+IW_DEV float unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
+// Rank of (value, id): larger is better, the lower id first.
+IW_DEV uint64_t key_of(float v, uint32_t id) { return ((uint64_t)order(v) << 32) | (uint32_t)~id; }
 
 template <typename F, typename T>
-IW_DEV T lp_block_reduce(T v, F f, T *red) {
+IW_DEV T block_reduce(T v, F f, T *red) {
     __syncthreads();
+#pragma unroll
     for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = red[0];
-    for (int w = 1; w < kLpThreads / 32; ++w) v = f(v, red[w]);
+    v = red[threadIdx.x & (kWarps - 1)];
+#pragma unroll
+    for (int o = kWarps / 2; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
+// A row cut into 16-byte vectors: `head` elements before the first aligned one,
+// `vecs` vectors, `tail` elements. Vector v belongs to thread v % kThreads,
+// head and tail element e to thread e (they are fewer than 16).
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) token_logprobs_kernel(LogprobsArgs a) {
+struct Row {
+    static constexpr int kPer = 16 / sizeof(T);
+    const T *x;
+    int V, head, vecs, tail;
+    IW_DEV Row(const T *x_, int V_) : x(x_), V(V_) {
+        const int misaligned = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+        head = min(V, misaligned ? kPer - misaligned : 0);
+        vecs = (V - head) / kPer;
+        tail = V - head - vecs * kPer;
+    }
+    IW_DEV int first(int v) const { return head + v * kPer; }
+    IW_DEV int4 load(int v) const { return *reinterpret_cast<const int4 *>(x + first(v)); }
+    // index of the thread's element outside the vectors, -1 for none
+    IW_DEV int edge(int t) const { return t < head ? t : (t < head + tail ? t + vecs * kPer : -1); }
+};
+
+// kPer suppression bits from element i on.
+template <int N>
+IW_DEV uint32_t bits_at(const uint32_t *bits, int i, int V) {
+    const int w = i >> 5, last = (V - 1) >> 5;
+    return __funnelshift_r(__ldg(bits + w), __ldg(bits + min(w + 1, last)), i & 31) & ((1u << N) - 1);
+}
+
+template <typename T>
+struct Shared {
+    float red[kWarps];
+    uint64_t red64[kWarps];
+    uint64_t cand[kCandidates];
+    uint16_t owners[kThreads];
+    int n_cand, n_owners;
+};
+
+template <typename T, bool SUP>
+__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArgs a) {
+    constexpr bool kBytes = sizeof(T) == 1;
+    constexpr int P = Row<T>::kPer;
     pdl_wait();
     pdl_launch();
-    __shared__ uint64_t red_k[kLpThreads / 32];
-    __shared__ float red_f[kLpThreads / 32];
+    extern __shared__ uint32_t hist[];  // int8: [256][32]
+    __shared__ Shared<T> s;
+    __shared__ uint32_t s_scan[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = blockIdx.x;
-    const T *x = reinterpret_cast<const T *>(a.x) + n * a.ld;
-    auto gone = [&](int64_t i) { return a.suppress && ((a.suppress[i >> 5] >> (i & 31)) & 1u); };
-    auto most = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
+    const Row<T> row(reinterpret_cast<const T *>(a.x) + n * a.ld, a.V);
+    auto gone = [&](int i) { return SUP && ((__ldg(a.suppress + (i >> 5)) >> (i & 31)) & 1u); };
+    auto most = [](float p, float q) { return fmaxf(p, q); };
     auto add = [](float p, float q) { return p + q; };
-    uint64_t best = 0;
-    float bad = 0.f;
-    for (int i = threadIdx.x; i < a.V; i += kLpThreads) {
-        if (gone(i)) continue;
-        const float v = lp_float(x[i]);
-        if (!(v < INFINITY)) bad = 1.f;
-        else if (v > -INFINITY) best = most(best, lp_key(v, i));
+    const float c = a.scale * 1.4426950408889634f;  // scale / ln 2
+    if (tid == 0) s.n_cand = s.n_owners = 0;
+
+    float mine = -INFINITY;   // the thread's largest logit
+    float m, S, W;            // of the row: maximum (unscaled), sum of 2^t, sum of t 2^t with t = c (x - m)
+    uint32_t at_least = 0;    // elements that reach the threshold (int8)
+    uint32_t threshold = 0;   // order() of the smallest value that may be among the best
+    if constexpr (kBytes) {
+        for (int i = tid; i < 256 * 32 / 4; i += kThreads) reinterpret_cast<int4 *>(hist)[i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        const uint32_t column = (uint32_t)__cvta_generic_to_shared(hist) + lane * 4;
+        uint32_t even = 0, odd = 0;  // largest x + 128 of the bytes 0, 2 and 1, 3, 16 bits each
+        auto count = [&](uint32_t u) { asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(column + u * 128)); };
+        auto words = [&](uint32_t w, uint32_t x, uint32_t sup) {
+            w ^= 0x80808080u, x ^= 0x80808080u;
+            if (!SUP || sup == 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) count(__byte_perm(w, 0, 0x4440 + e));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) count(__byte_perm(x, 0, 0x4440 + e));
+                even = __vimax3_u16x2(even, w & 0x00ff00ffu, x & 0x00ff00ffu);
+                odd = __vimax3_u16x2(odd, __byte_perm(w, 0, 0x4341), __byte_perm(x, 0, 0x4341));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (!((sup >> e) & 1)) {
+                        const uint32_t u = __byte_perm(e < 4 ? w : x, 0, 0x4440 + (e & 3));
+                        count(u);
+                        even = __vimax3_u16x2(even, u, 0);
+                    }
+            }
+        };
+        for (int v = tid; v < row.vecs; v += kThreads) {
+            const int4 w = row.load(v);
+            uint32_t sup = 0;
+            if (SUP) sup = bits_at<16>(a.suppress, row.first(v), a.V);
+            words(w.x, w.y, sup & 255), words(w.z, w.w, sup >> 8);
+        }
+        const int e = row.edge(tid);
+        const bool extra = e >= 0 && !gone(e);
+        if (extra) {
+            const uint32_t u = (uint32_t)((int)row.x[e] + 128);
+            count(u);
+            even = __vimax3_u16x2(even, u, 0);
+        }
+        mine = (float)(int)max(max(even & 0xffffu, even >> 16), max(odd & 0xffffu, odd >> 16)) - 128.f;
+        __syncthreads();
+        // bin 255 - tid: counts from the largest value down
+        uint32_t cnt = 0;
+        if (tid < 256)
+#pragma unroll 8
+            for (int j = 0; j < 32; ++j) cnt += hist[(255 - tid) * 32 + ((j + lane) & 31)];
+        uint32_t sum = cnt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t t = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += t;
+        }
+        if (lane == 31 && tid < 256) s_scan[warp] = sum;
+        m = block_reduce(cnt ? 127.f - tid : -INFINITY, most, s.red);
+        if (tid < 256)
+            for (int w = 0; w < warp; ++w) sum += s_scan[w];
+        const float t = c * (127.f - tid - m), ex = cnt ? (float)cnt * exp2f(t) : 0.f;
+        S = block_reduce(ex, add, s.red);
+        W = block_reduce(cnt ? ex * t : 0.f, add, s.red);
+        if (a.top > 0 && m > -INFINITY) {
+            // the value at which the count first reaches `top` (the smallest there is, if it never does)
+            const bool reach = tid < 256 && cnt && sum >= (uint32_t)a.top && sum - cnt < (uint32_t)a.top;
+            const float v = block_reduce(reach ? 127.f - tid : -INFINITY, most, s.red);
+            const float low = v > -INFINITY ? v : -128.f;
+            at_least = (uint32_t)block_reduce(tid < 256 && 127.f - tid == low ? (float)sum : 0.f, most, s.red);
+            threshold = order(low);
+        }
+    } else {
+        float Sm = 0.f, Wm = 0.f;
+        auto take = [&](const float (&v)[P]) {
+            float top = v[0];
+#pragma unroll
+            for (int e = 1; e < P; ++e) top = fmaxf(top, v[e]);
+            if (top > mine) {
+                const float d = Sm != 0.f ? fmaxf(c * (mine - top), -200.f) : 0.f;  // nothing to rescale yet: Sm == 0
+                const float f = exp2_approx(d);
+                Wm = (Wm + d * Sm) * f;
+                Sm *= f;
+                mine = top;
+            }
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                // far below the maximum, or -inf: 2^-200; a NaN passes as NaN
+                const float d = c * (v[e] - mine), t = d < -200.f ? -200.f : d, ex = exp2_approx(t);
+                Sm += ex;
+                Wm = fmaf(ex, t, Wm);
+            }
+        };
+        for (int v = tid; v < row.vecs; v += kThreads) {
+            const int4 w = row.load(v);
+            float f[P];
+            if constexpr (sizeof(T) == 4) {
+                f[0] = __int_as_float(w.x), f[1] = __int_as_float(w.y), f[2] = __int_as_float(w.z), f[3] = __int_as_float(w.w);
+            } else {
+                const uint32_t q[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    T lo, hi;
+                    *reinterpret_cast<uint16_t *>(&lo) = (uint16_t)q[e];
+                    *reinterpret_cast<uint16_t *>(&hi) = (uint16_t)(q[e] >> 16);
+                    f[2 * e] = to_float(lo), f[2 * e + 1] = to_float(hi);
+                }
+            }
+            if (SUP) {
+                const uint32_t sup = bits_at<P>(a.suppress, row.first(v), a.V);
+                if (sup) {
+#pragma unroll
+                    for (int e = 0; e < P; ++e)
+                        if ((sup >> e) & 1) f[e] = -INFINITY;
+                }
+            }
+            // a vector of -inf before anything else adds nothing (and has no maximum to be relative to)
+            bool some = mine > -INFINITY;
+#pragma unroll
+            for (int e = 0; e < P; ++e) some |= !(f[e] == -INFINITY);
+            if (some) take(f);
+        }
+        const int e = row.edge(tid);
+        if (e >= 0 && !gone(e)) {
+            float f[P];
+            f[0] = to_float(row.x[e]);
+#pragma unroll
+            for (int k = 1; k < P; ++k) f[k] = -INFINITY;
+            if (!(f[0] == -INFINITY)) take(f);
+        }
+        m = block_reduce(mine, most, s.red);
+        const float d = mine > -INFINITY ? fmaxf(c * (mine - m), -200.f) : 0.f, f = exp2_approx(d);
+        S = block_reduce(Sm * f, add, s.red);
+        W = block_reduce((Wm + d * Sm) * f, add, s.red);
     }
-    bad = lp_block_reduce(bad, add, red_f);
-    best = lp_block_reduce(best, most, red_k);
-    const float m = best ? lp_key_value(best) * a.scale : 0.f;
-    float S = 0.f, W = 0.f;
-    for (int i = threadIdx.x; i < a.V; i += kLpThreads) {
-        if (gone(i)) continue;
-        const float d = lp_float(x[i]) * a.scale - m;
-        const float e = expf(d);
-        S += e;
-        if (e > 0.f) W += e * d;
-    }
-    S = lp_block_reduce(S, add, red_f);
-    W = lp_block_reduce(W, add, red_f);
-    const float ln = logf(S);
-    const bool is_bad = bad > 0.f, none = best == 0;
-    if (threadIdx.x == 0) a.entropy[n] = is_bad ? NAN : (none ? 0.f : ln - W / S);
-    for (int64_t c = threadIdx.x; c < a.C; c += kLpThreads) {
-        const int64_t t = a.targets[n * a.C + c];
+    // a NaN makes S NaN, and so does +inf, from which nothing finite can be taken
+    const bool bad = !(S >= 0.f) || m == INFINITY;
+    const bool none = !bad && m == -INFINITY;
+    const float log2S = log2f(S);
+    constexpr float kLn2 = 0.6931471805599453f;
+    auto log_prob = [&](float x) { return a.scale * (x - m) - kLn2 * log2S; };
+    if (tid == 0) a.entropy[n] = bad ? NAN : (none ? 0.f : kLn2 * (log2S - W / S));
+    for (int64_t k = tid; k < a.C; k += kThreads) {
+        const int64_t t = a.targets[n * a.C + k];
         float r;
         if (t < 0) r = 0.f;
-        else if (t >= a.V || is_bad) r = NAN;
-        else if (none || gone(t)) r = -INFINITY;
-        else r = lp_float(x[t]) * a.scale - m - ln;
-        a.lp[n * a.C + c] = r;
+        else if (t >= a.V || bad) r = NAN;
+        else if (none || gone((int)t) || !(to_float(row.x[t]) > -INFINITY)) r = -INFINITY;
+        else r = log_prob(to_float(row.x[t]));
+        a.lp[n * a.C + k] = r;
     }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-        uint64_t next = 0;
-        if (!is_bad)
-            for (int i = threadIdx.x; i < a.V; i += kLpThreads) {
-                const float v = lp_float(x[i]);
-                if (gone(i) || !(v > -INFINITY)) continue;
-                const uint64_t key = lp_key(v, i);
-                if (key < last) next = most(next, key);
-            }
-        next = lp_block_reduce(next, most, red_k);
-        if (threadIdx.x == 0) {
-            a.top_ids[n * a.top + k] = next ? (int64_t)(uint32_t)~(uint32_t)next : -1;
-            a.top_lp[n * a.top + k] = is_bad ? NAN : (next ? lp_key_value(next) * a.scale - m - ln : -INFINITY);
+    if (a.top == 0) return;
+    int64_t *ids = a.top_ids + n * a.top;
+    float *lps = a.top_lp + n * a.top;
+    if (bad || none) {
+        for (int k = tid; k < a.top; k += kThreads) ids[k] = -1, lps[k] = bad ? NAN : -INFINITY;
+        return;
+    }
+    bool slow = false;
+    if constexpr (kBytes) {
+        slow = at_least > kCandidates;
+    } else {
+        // the largest 16-bit prefix that the maxima of `top` threads reach
+        const uint32_t o = mine > -INFINITY ? order(mine) >> 16 : 0;
+        uint32_t p = 0;
+#pragma unroll 1
+        for (int b = 15; b >= 0; --b)
+            if (__syncthreads_count(o >= (p | (1u << b))) >= a.top) p |= 1u << b;
+        threshold = p << 16;
+    }
+    if (!slow) {
+        if (mine > -INFINITY && order(mine) >= threshold) s.owners[atomicAdd(&s.n_owners, 1)] = (uint16_t)tid;
+        __syncthreads();
+        auto offer = [&](int i) {
+            const float v = to_float(row.x[i]);
+            if (!(v > -INFINITY) || order(v) < threshold || gone(i)) return;
+            const int at = atomicAdd(&s.n_cand, 1);
+            if (at < kCandidates) s.cand[at] = key_of(v, i);
+        };
+        // a warp per such thread: its lanes take the thread's vectors
+        const int owners = s.n_owners;
+        for (int k = warp; k < owners; k += kWarps) {
+            const int t = s.owners[k];
+            for (int v = t + lane * kThreads; v < row.vecs; v += 32 * kThreads)
+#pragma unroll 1
+                for (int e = 0; e < P; ++e) offer(row.first(v) + e);
+            if (lane == 0 && row.edge(t) >= 0) offer(row.edge(t));
         }
-        last = next;
+        __syncthreads();
+        const int found = s.n_cand;
+        slow = found > kCandidates;
+        if (!slow) {
+            for (int k = tid; k < max(found, a.top); k += kThreads) {
+                if (k >= found) {
+                    if (k < a.top) ids[k] = -1, lps[k] = -INFINITY;
+                    continue;
+                }
+                const uint64_t key = s.cand[k];
+                int rank = 0;
+                for (int j = 0; j < found; ++j) rank += s.cand[j] > key;
+                if (rank < a.top) {
+                    ids[rank] = (int64_t)(uint32_t)~(uint32_t)key;
+                    lps[rank] = log_prob(unorder((uint32_t)(key >> 32)));
+                }
+            }
+        }
+    }
+    if (slow) {
+        uint64_t last = ~0ull;
+        for (int k = 0; k < a.top; ++k) {
+            uint64_t next = 0;
+            for (int i = tid; i < a.V; i += kThreads) {
+                const float v = to_float(row.x[i]);
+                if (gone(i) || !(v > -INFINITY)) continue;
+                const uint64_t key = key_of(v, i);
+                if (key < last && key > next) next = key;
+            }
+            next = block_reduce(next, [](uint64_t p, uint64_t q) { return p > q ? p : q; }, s.red64);
+            if (tid == 0) {
+                ids[k] = next ? (int64_t)(uint32_t)~(uint32_t)next : -1;
+                lps[k] = next ? log_prob(unorder((uint32_t)(next >> 32))) : -INFINITY;
+            }
+            last = next;
+        }
     }
 }
 
+template <typename T>
+static cudaError_t launch(const LogprobsArgs &a, cudaStream_t st) {
+    const size_t smem = sizeof(T) == 1 ? 256 * 32 * 4 : 0;
+    const dim3 grid((unsigned)a.N), block(kThreads);
+    return a.suppress ? launch_pdl(token_logprobs_kernel<T, true>, grid, block, smem, st, a)
+                      : launch_pdl(token_logprobs_kernel<T, false>, grid, block, smem, st, a);
+}
+
+}  // namespace lp
+
 cudaError_t token_logprobs(const LogprobsArgs &a, cudaStream_t st) {
-    const dim3 grid((unsigned)a.N), block(kLpThreads);
     switch (a.dtype) {
-        case 0: return launch_pdl(token_logprobs_kernel<int8_t>, grid, block, 0, st, a);
-        case 1: return launch_pdl(token_logprobs_kernel<__half>, grid, block, 0, st, a);
-        case 2: return launch_pdl(token_logprobs_kernel<__nv_bfloat16>, grid, block, 0, st, a);
-        default: return launch_pdl(token_logprobs_kernel<float>, grid, block, 0, st, a);
+        case 0: return lp::launch<int8_t>(a, st);
+        case 1: return lp::launch<__half>(a, st);
+        case 2: return lp::launch<__nv_bfloat16>(a, st);
+        default: return lp::launch<float>(a, st);
     }
 }
 

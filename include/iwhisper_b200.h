@@ -523,8 +523,8 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream);
 typedef struct iw_token_logprobs_desc {
     const void *logits; int64_t ld;      /* [N, V] at a row stride of ld elements     */
     int dtype;                           /* IW_LOGITS_*                               */
-    int64_t N, V;
-    float scale;                         /* > 0: the logit of x is scale * x          */
+    int64_t N, V;                        /* V <= 2^30                                 */
+    float scale;                         /* in (0, 1e30]: the logit of x is scale * x  */
     const uint32_t *suppress_bits;       /* optional [ceil(V/32)]: bit id%32 of word id/32 removes id */
     const int64_t *targets; int64_t C;   /* [N, C] given tokens                       */
     int64_t top;                         /* alternatives per row, <= min(V, IW_LOGPROBS_MAX_TOP) */
