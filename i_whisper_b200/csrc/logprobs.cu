@@ -25,8 +25,11 @@
 namespace iw {
 namespace lp {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kCandidates = 512;
+// Threads per block: int8 rows want few, since each block sums and reads its
+// histogram once; the others want many loads in flight.
+template <typename T>
+constexpr int threads_of() { return sizeof(T) == 1 ? 256 : 512; }
 
 IW_DEV float to_float(int8_t v) { return (float)v; }
 IW_DEV float to_float(float v) { return v; }
@@ -48,8 +51,9 @@ IW_DEV float unorder(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o
 // Rank of (value, id): larger is better, the lower id first.
 IW_DEV uint64_t key_of(float v, uint32_t id) { return ((uint64_t)order(v) << 32) | (uint32_t)~id; }
 
-template <typename F, typename T>
+template <int kThreads, typename F, typename T>
 IW_DEV T block_reduce(T v, F f, T *red) {
+    constexpr int kWarps = kThreads / 32;
     __syncthreads();
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -62,7 +66,7 @@ IW_DEV T block_reduce(T v, F f, T *red) {
 }
 
 // A row cut into 16-byte vectors: `head` elements before the first aligned one,
-// `vecs` vectors, `tail` elements. Vector v belongs to thread v % kThreads,
+// `vecs` vectors, `tail` elements. Vector v belongs to thread v % (threads),
 // head and tail element e to thread e (they are fewer than 16).
 template <typename T>
 struct Row {
@@ -88,24 +92,32 @@ IW_DEV uint32_t bits_at(const uint32_t *bits, int i, int V) {
     return __funnelshift_r(__ldg(bits + w), __ldg(bits + min(w + 1, last)), i & 31) & ((1u << N) - 1);
 }
 
-template <typename T>
+template <int kThreads>
 struct Shared {
-    float red[kWarps];
-    uint64_t red64[kWarps];
+    float red[kThreads / 32];
+    uint64_t red64[kThreads / 32];
     uint64_t cand[kCandidates];
     uint16_t owners[kThreads];
     int n_cand, n_owners;
+    uint32_t bins[256], at_least, threshold;  // int8
+    float m, S, W;
 };
 
+// Larger of two, NaN when either is.
+IW_DEV float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 template <typename T, bool SUP>
-__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArgs a) {
+__global__ void __launch_bounds__(threads_of<T>(), sizeof(T) == 1 ? 5 : 3) token_logprobs_kernel(LogprobsArgs a) {
     constexpr bool kBytes = sizeof(T) == 1;
-    constexpr int P = Row<T>::kPer;
+    constexpr int P = Row<T>::kPer, kThreads = threads_of<T>(), kWarps = kThreads / 32;
     pdl_wait();
     pdl_launch();
     extern __shared__ uint32_t hist[];  // int8: [256][32]
-    __shared__ Shared<T> s;
-    __shared__ uint32_t s_scan[8];
+    __shared__ Shared<kThreads> s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = blockIdx.x;
     const Row<T> row(reinterpret_cast<const T *>(a.x) + n * a.ld, a.V);
@@ -159,49 +171,80 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArg
         }
         mine = (float)(int)max(max(even & 0xffffu, even >> 16), max(odd & 0xffffu, odd >> 16)) - 128.f;
         __syncthreads();
-        // bin 255 - tid: counts from the largest value down
-        uint32_t cnt = 0;
-        if (tid < 256)
-#pragma unroll 8
-            for (int j = 0; j < 32; ++j) cnt += hist[(255 - tid) * 32 + ((j + lane) & 31)];
-        uint32_t sum = cnt;
+        {  // a thread per value; its 32 counters in an order free of bank conflicts
+            uint32_t cnt = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t t = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += t;
+            for (int j = 0; j < 8; ++j) {
+                const uint4 q = reinterpret_cast<const uint4 *>(hist)[tid * 8 + ((j + lane) & 7)];
+                cnt += q.x + q.y + q.z + q.w;
+            }
+            s.bins[255 - tid] = cnt;  // from the largest value down
         }
-        if (lane == 31 && tid < 256) s_scan[warp] = sum;
-        m = block_reduce(cnt ? 127.f - tid : -INFINITY, most, s.red);
-        if (tid < 256)
-            for (int w = 0; w < warp; ++w) sum += s_scan[w];
-        const float t = c * (127.f - tid - m), ex = cnt ? (float)cnt * exp2f(t) : 0.f;
-        S = block_reduce(ex, add, s.red);
-        W = block_reduce(cnt ? ex * t : 0.f, add, s.red);
-        if (a.top > 0 && m > -INFINITY) {
-            // the value at which the count first reaches `top` (the smallest there is, if it never does)
-            const bool reach = tid < 256 && cnt && sum >= (uint32_t)a.top && sum - cnt < (uint32_t)a.top;
-            const float v = block_reduce(reach ? 127.f - tid : -INFINITY, most, s.red);
-            const float low = v > -INFINITY ? v : -128.f;
-            at_least = (uint32_t)block_reduce(tid < 256 && 127.f - tid == low ? (float)sum : 0.f, most, s.red);
-            threshold = order(low);
+        __syncthreads();
+        if (warp == 0) {  // lane: the values 127 - 8 * lane .. 120 - 8 * lane
+            uint32_t cnt[8], sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum += cnt[j] = s.bins[8 * lane + j];
+            uint32_t upto = sum;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += t;
+            }
+            int top = -1000;
+#pragma unroll
+            for (int j = 7; j >= 0; --j)
+                if (cnt[j]) top = 127 - 8 * lane - j;
+            top = __reduce_max_sync(0xffffffffu, top);
+            float Sm = 0.f, Wm = 0.f;
+            // the value at which the count first reaches `top` (-128 if it never does)
+            uint32_t before = upto - sum, reached = 0;
+            int low = -128;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int value = 127 - 8 * lane - j;
+                if (cnt[j]) {
+                    const float t = c * (float)(value - top), ex = (float)cnt[j] * exp2f(t);
+                    Sm += ex;
+                    Wm = fmaf(ex, t, Wm);
+                }
+                if (before < (uint32_t)a.top && before + cnt[j] >= (uint32_t)a.top) low = value, reached = before + cnt[j];
+                before += cnt[j];
+            }
+            const uint32_t total = __shfl_sync(0xffffffffu, upto, 31);
+            low = __reduce_max_sync(0xffffffffu, low);
+            reached = __reduce_max_sync(0xffffffffu, reached);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                Sm += __shfl_xor_sync(0xffffffffu, Sm, o);
+                Wm += __shfl_xor_sync(0xffffffffu, Wm, o);
+            }
+            if (lane == 0) {
+                s.m = total ? (float)top : -INFINITY;
+                s.S = Sm, s.W = Wm;
+                s.at_least = reached ? reached : total;
+                s.threshold = order((float)low);
+            }
         }
+        __syncthreads();
+        m = s.m, S = s.S, W = s.W;
+        at_least = s.at_least, threshold = s.threshold;
     } else {
-        float Sm = 0.f, Wm = 0.f;
+        float Sm = 0.f, Wm = 0.f, ref = 0.f;  // ref: mine, or 0 before there is one
         auto take = [&](const float (&v)[P]) {
             float top = v[0];
 #pragma unroll
             for (int e = 1; e < P; ++e) top = fmaxf(top, v[e]);
             if (top > mine) {
-                const float d = Sm != 0.f ? fmaxf(c * (mine - top), -200.f) : 0.f;  // nothing to rescale yet: Sm == 0
-                const float f = exp2_approx(d);
+                const float d = mine > -INFINITY ? fmaxf(c * (mine - top), -200.f) : 0.f, f = exp2_approx(d);
                 Wm = (Wm + d * Sm) * f;
                 Sm *= f;
-                mine = top;
+                mine = ref = top;
             }
 #pragma unroll
             for (int e = 0; e < P; ++e) {
-                // far below the maximum, or -inf: 2^-200; a NaN passes as NaN
-                const float d = c * (v[e] - mine), t = d < -200.f ? -200.f : d, ex = exp2_approx(t);
+                // far below the maximum, or -inf: 2^-200, which is 0; a NaN passes as NaN
+                const float t = max_nan(c * (v[e] - ref), -200.f), ex = exp2_approx(t);
                 Sm += ex;
                 Wm = fmaf(ex, t, Wm);
             }
@@ -229,11 +272,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArg
                         if ((sup >> e) & 1) f[e] = -INFINITY;
                 }
             }
-            // a vector of -inf before anything else adds nothing (and has no maximum to be relative to)
-            bool some = mine > -INFINITY;
-#pragma unroll
-            for (int e = 0; e < P; ++e) some |= !(f[e] == -INFINITY);
-            if (some) take(f);
+            take(f);
         }
         const int e = row.edge(tid);
         if (e >= 0 && !gone(e)) {
@@ -241,12 +280,12 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArg
             f[0] = to_float(row.x[e]);
 #pragma unroll
             for (int k = 1; k < P; ++k) f[k] = -INFINITY;
-            if (!(f[0] == -INFINITY)) take(f);
+            take(f);
         }
-        m = block_reduce(mine, most, s.red);
+        m = block_reduce<kThreads>(mine, most, s.red);
         const float d = mine > -INFINITY ? fmaxf(c * (mine - m), -200.f) : 0.f, f = exp2_approx(d);
-        S = block_reduce(Sm * f, add, s.red);
-        W = block_reduce((Wm + d * Sm) * f, add, s.red);
+        S = block_reduce<kThreads>(Sm * f, add, s.red);
+        W = block_reduce<kThreads>((Wm + d * Sm) * f, add, s.red);
     }
     // a NaN makes S NaN, and so does +inf, from which nothing finite can be taken
     const bool bad = !(S >= 0.f) || m == INFINITY;
@@ -330,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArg
                 const uint64_t key = key_of(v, i);
                 if (key < last && key > next) next = key;
             }
-            next = block_reduce(next, [](uint64_t p, uint64_t q) { return p > q ? p : q; }, s.red64);
+            next = block_reduce<kThreads>(next, [](uint64_t p, uint64_t q) { return p > q ? p : q; }, s.red64);
             if (tid == 0) {
                 ids[k] = next ? (int64_t)(uint32_t)~(uint32_t)next : -1;
                 lps[k] = next ? log_prob(unorder((uint32_t)(next >> 32))) : -INFINITY;
@@ -343,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(LogprobsArg
 template <typename T>
 static cudaError_t launch(const LogprobsArgs &a, cudaStream_t st) {
     const size_t smem = sizeof(T) == 1 ? 256 * 32 * 4 : 0;
-    const dim3 grid((unsigned)a.N), block(kThreads);
+    const dim3 grid((unsigned)a.N), block(threads_of<T>());
     return a.suppress ? launch_pdl(token_logprobs_kernel<T, true>, grid, block, smem, st, a)
                       : launch_pdl(token_logprobs_kernel<T, false>, grid, block, smem, st, a);
 }
