@@ -26,15 +26,28 @@ namespace iw {
 namespace lp {
 
 constexpr int kCandidates = 512;
-// Threads per block: int8 rows want few, since each block sums and reads its
-// histogram once; the others want many loads in flight.
+// Threads per block where the rows fill the GPU: int8 rows want few, since each
+// block zeroes and sums its histogram once (4096 rows: 78 us with 256, 97 with
+// 512), the others 512 (bf16: 110 us with 256). Fewer rows than SMs leave
+// room for 1024 each.
 template <typename T>
 constexpr int threads_of() { return sizeof(T) == 1 ? 256 : 512; }
+constexpr int kThreadsFewRows = 1024;
 
 IW_DEV float to_float(int8_t v) { return (float)v; }
 IW_DEV float to_float(float v) { return v; }
 IW_DEV float to_float(__half v) { return __half2float(v); }
 IW_DEV float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// Two 16-bit floats of a word.
+IW_DEV void widen(__nv_bfloat16, uint32_t w, float &lo, float &hi) {
+    lo = __uint_as_float(w << 16);
+    hi = __uint_as_float(w & 0xffff0000u);
+}
+IW_DEV void widen(__half, uint32_t w, float &lo, float &hi) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    lo = v.x, hi = v.y;
+}
 
 IW_DEV float exp2_approx(float x) {
     float y;
@@ -110,10 +123,10 @@ IW_DEV float max_nan(float a, float b) {
     return d;
 }
 
-template <typename T, bool SUP>
-__global__ void __launch_bounds__(threads_of<T>(), sizeof(T) == 1 ? 5 : 3) token_logprobs_kernel(LogprobsArgs a) {
+template <typename T, bool SUP, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) == 1 ? 6 : 4)) token_logprobs_kernel(LogprobsArgs a) {
     constexpr bool kBytes = sizeof(T) == 1;
-    constexpr int P = Row<T>::kPer, kThreads = threads_of<T>(), kWarps = kThreads / 32;
+    constexpr int P = Row<T>::kPer, kWarps = kThreads / 32;
     pdl_wait();
     pdl_launch();
     extern __shared__ uint32_t hist[];  // int8: [256][32]
@@ -173,12 +186,14 @@ __global__ void __launch_bounds__(threads_of<T>(), sizeof(T) == 1 ? 5 : 3) token
         __syncthreads();
         {  // a thread per value; its 32 counters in an order free of bank conflicts
             uint32_t cnt = 0;
+            if (tid < 256) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint4 q = reinterpret_cast<const uint4 *>(hist)[tid * 8 + ((j + lane) & 7)];
-                cnt += q.x + q.y + q.z + q.w;
+                for (int j = 0; j < 8; ++j) {
+                    const uint4 q = reinterpret_cast<const uint4 *>(hist)[tid * 8 + ((j + lane) & 7)];
+                    cnt += q.x + q.y + q.z + q.w;
+                }
+                s.bins[255 - tid] = cnt;  // from the largest value down
             }
-            s.bins[255 - tid] = cnt;  // from the largest value down
         }
         __syncthreads();
         if (warp == 0) {  // lane: the values 127 - 8 * lane .. 120 - 8 * lane
@@ -257,12 +272,7 @@ __global__ void __launch_bounds__(threads_of<T>(), sizeof(T) == 1 ? 5 : 3) token
             } else {
                 const uint32_t q[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    T lo, hi;
-                    *reinterpret_cast<uint16_t *>(&lo) = (uint16_t)q[e];
-                    *reinterpret_cast<uint16_t *>(&hi) = (uint16_t)(q[e] >> 16);
-                    f[2 * e] = to_float(lo), f[2 * e + 1] = to_float(hi);
-                }
+                for (int e = 0; e < 4; ++e) widen(T(), q[e], f[2 * e], f[2 * e + 1]);
             }
             if (SUP) {
                 const uint32_t sup = bits_at<P>(a.suppress, row.first(v), a.V);
@@ -379,12 +389,16 @@ __global__ void __launch_bounds__(threads_of<T>(), sizeof(T) == 1 ? 5 : 3) token
     }
 }
 
+template <typename T, int kThreads>
+static cudaError_t launch_threads(const LogprobsArgs &a, cudaStream_t st) {
+    const size_t smem = sizeof(T) == 1 ? 256 * 32 * 4 : 0;
+    const dim3 grid((unsigned)a.N), block(kThreads);
+    return a.suppress ? launch_pdl(token_logprobs_kernel<T, true, kThreads>, grid, block, smem, st, a)
+                      : launch_pdl(token_logprobs_kernel<T, false, kThreads>, grid, block, smem, st, a);
+}
 template <typename T>
 static cudaError_t launch(const LogprobsArgs &a, cudaStream_t st) {
-    const size_t smem = sizeof(T) == 1 ? 256 * 32 * 4 : 0;
-    const dim3 grid((unsigned)a.N), block(threads_of<T>());
-    return a.suppress ? launch_pdl(token_logprobs_kernel<T, true>, grid, block, smem, st, a)
-                      : launch_pdl(token_logprobs_kernel<T, false>, grid, block, smem, st, a);
+    return a.N <= num_sms() ? launch_threads<T, kThreadsFewRows>(a, st) : launch_threads<T, threads_of<T>()>(a, st);
 }
 
 }  // namespace lp
