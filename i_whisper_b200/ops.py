@@ -13,7 +13,8 @@ are read with ``.item()``; the model runner caches them on the host instead.
 """
 from __future__ import annotations
 
-import ctypes as C
+import ctypes
+import struct
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -43,6 +44,11 @@ def _p(t: Optional[torch.Tensor]):
 
 def _stream():
     return torch.cuda.current_stream().cuda_stream
+
+
+# the current stream's handle without a torch.cuda.Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _scalar(t, name: str) -> int:
@@ -645,17 +651,43 @@ class PagedPlan(NamedTuple):
     tree_mask: Optional[torch.Tensor]  # [max_tokens, ceil(max_new/32)] int32 ancestor-or-self bits
 
 
-def _chk1(t, name: str, dtype: torch.dtype, n: int, at):
-    """A contiguous CUDA tensor [n] of `dtype` on the device of `at`."""
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or t.device != at or (n > 1 and t.stride(0) != 1):
-        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor [{n}] on {at}, got {t.dtype} {tuple(t.shape)} "
-                           f"on {t.device}")
+# The descriptors of these calls as packed bytes, laid out like the C structs: a
+# few times cheaper than filling a ctypes.Structure, and these calls are a step's
+# host time.
+_PLAN_DESC = struct.Struct("@PPqPqqPqPqqPqPPPPPPP")
+_ATTN_DESC = struct.Struct("@PqqPqPPqqqqqPqqPPPqqqqqqBbiBbi0q")
+_LOGP_DESC = struct.Struct("@PqiqqfPPqqPPPP")
+assert (_PLAN_DESC.size, _ATTN_DESC.size, _LOGP_DESC.size) == tuple(
+    ctypes.sizeof(d) for d in (_lib.PagedPlanDesc, _lib.TreeAttnDesc, _lib.TokenLogprobsDesc))
 
 
-def _chk_device(t, name: str):
-    """A CUDA tensor of the current device, whose stream the call uses."""
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+def _chk1(t, name: str, dtype: torch.dtype, n: int, device: int):
+    """A contiguous CUDA tensor [n] of `dtype` on CUDA device `device`."""
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous {dtype} tensor [{n}] on cuda:{device}, got {t.dtype} "
+                           f"{tuple(t.shape)} on {t.device}")
+
+
+def _chk_device(t, name: str) -> int:
+    """The index of a CUDA tensor's device, which has to be the current one (the call runs on its stream)."""
+    i = t.get_device()
+    if i < 0 or i != torch.cuda.current_device():
         raise RuntimeError(f"{name} must be on the current CUDA device, got {t.device}")
+    return i
+
+
+def _chk_table(t, device: int):
+    """Block table int32 [B, pages] with contiguous rows that do not overlap -> (B, pages, row stride)."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.get_device() != device:
+        raise RuntimeError("block_table must be an int32 CUDA tensor [B, pages] with contiguous rows")
+    (B, width), (ld, step) = t.shape, t.stride()
+    if width > 1 and step != 1:
+        raise RuntimeError("block_table must be an int32 CUDA tensor [B, pages] with contiguous rows")
+    if B <= 1:
+        ld = width
+    elif ld < width:
+        raise RuntimeError("block_table rows must not overlap")
+    return B, width, ld
 
 
 def paged_plan_cuda(context_lens, new_lens, block_table, free_pages, free_head, page_size: int, max_tokens: int,
@@ -671,50 +703,47 @@ def paged_plan_cuda(context_lens, new_lens, block_table, free_pages, free_head, 
     context) the new tokens form trees of at most ``max_new`` tokens, and the
     plan holds their ancestor masks. Nothing is read on the host: what does
     not fit is reported in ``status``."""
-    _chk_device(context_lens, "context_lens")
-    at = context_lens.device
-    B = context_lens.shape[0] if context_lens.dim() == 1 else -1
-    _chk1(context_lens, "context_lens", torch.int32, B, at)
-    _chk1(new_lens, "new_lens", torch.int32, B, at)
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or block_table.device != at
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise RuntimeError("block_table must be an int32 CUDA tensor [B, pages] with contiguous rows")
-    _chk1(free_pages, "free_pages", torch.int32, free_pages.numel(), at)
-    _chk1(free_head, "free_head", torch.int32, 1, at)
-    width = block_table.shape[1]
-    if B > 1 and block_table.stride(0) < width:
-        raise RuntimeError("block_table rows must not overlap")
-    max_tokens = int(max_tokens)
+    dev = _chk_device(context_lens, "context_lens")
+    B, width, ld = _chk_table(block_table, dev)
+    _chk1(context_lens, "context_lens", torch.int32, B, dev)
+    _chk1(new_lens, "new_lens", torch.int32, B, dev)
+    n_free = free_pages.numel()
+    _chk1(free_pages, "free_pages", torch.int32, n_free, dev)
+    _chk1(free_head, "free_head", torch.int32, 1, dev)
     if max_tokens < 0:
         raise RuntimeError("max_tokens must not be negative")
     words = 0
     if parents is not None:
-        _chk1(parents, "parents", torch.int32, max_tokens, at)
+        _chk1(parents, "parents", torch.int32, max_tokens, dev)
         if max_new is None or max_new < 1:
             raise RuntimeError("parents need max_new, the most new tokens of a request")
         words = (max_new + 31) // 32
+    at = context_lens.device
     slots = torch.empty(max_tokens, dtype=torch.int64, device=at)
     ints = torch.empty(max_tokens * (2 + words) + B + 3, dtype=torch.int32, device=at)
-    mask, request, position, starts, head, status = ints.split(
-        [max_tokens * words, max_tokens, max_tokens, B + 1, 1, 1])
-    d = _lib.PagedPlanDesc(
-        context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(),
-        block_table.stride(0) if B > 1 else width, width, free_pages.data_ptr(), free_pages.shape[0], free_head.data_ptr(),
-        page_size, max_tokens, _p(parents), max_new or 0, slots.data_ptr(), request.data_ptr(), position.data_ptr(),
-        mask.data_ptr() if words else None, starts.data_ptr(), head.data_ptr(), status.data_ptr())
-    _lib.call("iw_paged_plan", C.byref(d), _stream())
+    mask, request, position, starts, head, status = ints.split_with_sizes(
+        (max_tokens * words, max_tokens, max_tokens, B + 1, 1, 1))
+    p = ints.data_ptr()
+    p_req = p + 4 * max_tokens * words
+    p_pos = p_req + 4 * max_tokens
+    p_starts = p_pos + 4 * max_tokens
+    p_head = p_starts + 4 * (B + 1)
+    _lib.call("iw_paged_plan", _PLAN_DESC.pack(
+        context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), ld, width, free_pages.data_ptr(), n_free,
+        free_head.data_ptr(), page_size, max_tokens, parents.data_ptr() if words else 0, max_new or 0, slots.data_ptr(),
+        p_req, p_pos, p if words else 0, p_starts, p_head, p_head + 4), _raw_stream(dev))
     return PagedPlan(slots, request, position, starts, head, status, mask.view(max_tokens, words) if words else None)
 
 
-def _cache_checks(k_cache, v_cache, at):
+def _cache_checks(k_cache, v_cache, device: int):
     """Paged K/V caches int8 [pages, heads, page_size, D] of one layout (D
     contiguous, any order of the other axes)."""
     if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
         raise RuntimeError("k_cache and v_cache must be int8")
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
         raise RuntimeError("k_cache and v_cache must be [pages, heads, page_size, D]")
-    if k_cache.device != at or v_cache.device != at:
-        raise RuntimeError(f"k_cache and v_cache must be on {at}")
+    if k_cache.get_device() != device or v_cache.get_device() != device:
+        raise RuntimeError(f"k_cache and v_cache must be on cuda:{device}")
     st = k_cache.stride()
     if st != v_cache.stride() or st[3] != 1:
         raise RuntimeError("k_cache and v_cache must have equal strides and contiguous rows")
@@ -726,19 +755,20 @@ def paged_kv_write_cuda(k, v, slots, k_cache, v_cache) -> None:
     of the fused projection's output may be passed as views) into the paged
     caches (int8 [pages, heads, page_size, D]) at ``slots`` (int64 [N],
     ``PagedPlan.slots``; rows with a negative slot are skipped), in place."""
-    _chk_device(k, "k")
-    if k.dtype != torch.int8 or v.dtype != torch.int8 or k.dim() != 3 or k.shape != v.shape or v.device != k.device:
+    dev = _chk_device(k, "k")
+    if k.dtype != torch.int8 or v.dtype != torch.int8 or k.dim() != 3 or k.shape != v.shape or v.get_device() != dev:
         raise RuntimeError("k and v must be int8 CUDA tensors [N, heads, D] of one shape")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    sk, sv = k.stride(), v.stride()
+    if sk[2] != 1 or sv[2] != 1:
         raise RuntimeError("k and v must have contiguous head rows")
     N, H, D = k.shape
-    st = _cache_checks(k_cache, v_cache, k.device)
-    if k_cache.shape[1] != H or k_cache.shape[3] != D:
+    st = _cache_checks(k_cache, v_cache, dev)
+    P, Hc, page, Dc = k_cache.shape
+    if Hc != H or Dc != D:
         raise RuntimeError(f"k_cache must have {H} heads of {D}, got {tuple(k_cache.shape)}")
-    _chk1(slots, "slots", torch.int64, N, k.device)
-    _lib.call("iw_paged_kv_write", k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-              slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], k_cache.shape[0],
-              k_cache.shape[2], N, H, D, _stream())
+    _chk1(slots, "slots", torch.int64, N, dev)
+    _lib.call("iw_paged_kv_write", k.data_ptr(), sk[0], sk[1], v.data_ptr(), sv[0], sv[1], slots.data_ptr(),
+              k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], P, page, N, H, D, _raw_stream(dev))
 
 
 def tree_attention_cuda(q, k_cache, v_cache, block_table, context_lens, starts, qk_multiplier, qk_shift, frac_bits,
@@ -753,40 +783,35 @@ def tree_attention_cuda(q, k_cache, v_cache, block_table, context_lens, starts, 
     without a mask itself and those before it. The caches may have fewer
     heads than q (query head h reads head h // (H / heads)). Rows from
     ``starts[B]`` on are padding and give 0."""
-    _chk_device(q, "q")
-    at = q.device
+    dev = _chk_device(q, "q")
     if q.dtype != torch.int8 or q.dim() != 3 or q.stride(2) != 1:
         raise RuntimeError("q must be an int8 CUDA tensor [N, H, D] with contiguous head rows")
     N, H, D = q.shape
-    st = _cache_checks(k_cache, v_cache, at)
+    st = _cache_checks(k_cache, v_cache, dev)
     P, Hkv, page, Dk = k_cache.shape
     if Dk != D:
         raise RuntimeError(f"head dimension mismatch: q has {D}, the caches {Dk}")
     if Hkv < 1 or H % Hkv:
         raise RuntimeError(f"the caches' head count {Hkv} must divide the query head count {H}")
-    if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != at
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
-        raise RuntimeError("block_table must be an int32 CUDA tensor [B, pages] with contiguous rows")
-    B, width = block_table.shape
-    _chk1(context_lens, "context_lens", torch.int32, B, at)
-    _chk1(starts, "starts", torch.int32, B + 1, at)
-    words = 0
+    B, width, ld = _chk_table(block_table, dev)
+    _chk1(context_lens, "context_lens", torch.int32, B, dev)
+    _chk1(starts, "starts", torch.int32, B + 1, dev)
+    p_mask = words = 0
     if tree_mask is not None:
         if (tree_mask.dtype != torch.int32 or tree_mask.dim() != 2 or tree_mask.shape[0] != N or tree_mask.shape[1] < 1
-                or tree_mask.device != at or not tree_mask.is_contiguous()):
+                or tree_mask.get_device() != dev or not tree_mask.is_contiguous()):
             raise RuntimeError("tree_mask must be a contiguous int32 CUDA tensor [N, words]")
-        words = tree_mask.shape[1]
+        p_mask, words = tree_mask.data_ptr(), tree_mask.shape[1]
     if out is None:
-        out = torch.empty(N, H * D, dtype=torch.int8, device=at)
-    elif out.dtype != torch.int8 or out.shape != (N, H * D) or out.device != at or out.stride(1) != 1:
+        out = torch.empty(N, H * D, dtype=torch.int8, device=q.device)
+    elif out.dtype != torch.int8 or out.shape != (N, H * D) or out.get_device() != dev or out.stride(1) != 1:
         raise RuntimeError(f"out must be an int8 CUDA tensor [{N}, {H * D}] with contiguous rows")
-    d = _lib.TreeAttnDesc(
+    _lib.call("iw_tree_attention", _ATTN_DESC.pack(
         q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
-        st[0], st[1], st[2], P, page, block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width,
-        context_lens.data_ptr(), starts.data_ptr(), _p(tree_mask), words, B, N, H, Hkv, D,
-        _scalar(qk_multiplier, "qk_multiplier"), _scalar(qk_shift, "qk_shift"), _scalar(frac_bits, "frac_bits"),
-        _scalar(av_multiplier, "av_multiplier"), _scalar(av_shift, "av_shift"), int(rsqrt_offset))
-    _lib.call("iw_tree_attention", C.byref(d), _stream())
+        st[0], st[1], st[2], P, page, block_table.data_ptr(), ld, width, context_lens.data_ptr(), starts.data_ptr(),
+        p_mask, words, B, N, H, Hkv, D, _scalar(qk_multiplier, "qk_multiplier"), _scalar(qk_shift, "qk_shift"),
+        _scalar(frac_bits, "frac_bits"), _scalar(av_multiplier, "av_multiplier"), _scalar(av_shift, "av_shift"),
+        rsqrt_offset), _raw_stream(dev))
     return out
 
 
@@ -804,31 +829,32 @@ def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, 
     [N, top], top_logprobs float32 [N, top]); equal logits are ordered by id,
     and an alternative that does not exist (fewer tokens than ``top`` with a
     logit above -inf) has id -1 and -inf. A row with a NaN or +inf gives NaN."""
-    _chk_device(logits, "logits")
-    at = logits.device
+    dev = _chk_device(logits, "logits")
     if logits.dtype not in _LOGITS:
         raise RuntimeError(f"logits must be int8, float16, bfloat16 or float32, got {logits.dtype}")
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError("logits must be [N, V] with contiguous rows")
     N, V = logits.shape
-    n_given = 0
+    n_given = p_targets = p_suppress = 0
     if targets is not None:
-        if (targets.dtype != torch.int64 or targets.dim() != 2 or targets.shape[0] != N or targets.device != at
+        if (targets.dtype != torch.int64 or targets.dim() != 2 or targets.shape[0] != N or targets.get_device() != dev
                 or not targets.is_contiguous()):
             raise RuntimeError("targets must be a contiguous int64 CUDA tensor [N, C]")
         n_given = targets.shape[1]
+        p_targets = targets.data_ptr() if n_given else 0
     if suppress_bits is not None:
         if suppress_bits.dtype not in (torch.int32, torch.uint32):
             raise RuntimeError(f"suppress_bits must be int32 or uint32, got {suppress_bits.dtype}")
-        _chk1(suppress_bits, "suppress_bits", suppress_bits.dtype, (V + 31) // 32, at)
+        _chk1(suppress_bits, "suppress_bits", suppress_bits.dtype, (V + 31) // 32, dev)
+        p_suppress = suppress_bits.data_ptr()
     if top < 0 or top > min(V, _lib.LOGPROBS_MAX_TOP):
         raise RuntimeError(f"top must be in [0, min(V, {_lib.LOGPROBS_MAX_TOP})], got {top}")
+    at = logits.device
     floats = torch.empty(N * (n_given + 1 + top), dtype=torch.float32, device=at)
-    lp, entropy, top_lp = floats.split([N * n_given, N, N * top])
+    lp, entropy, top_lp = floats.split_with_sizes((N * n_given, N, N * top))
     ids = torch.empty(N, top, dtype=torch.int64, device=at)
-    d = _lib.TokenLogprobsDesc(
-        logits.data_ptr(), logits.stride(0) if N > 1 else V, _LOGITS[logits.dtype], N, V, scale, _p(suppress_bits),
-        _p(targets) if n_given else None, n_given, top, lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(),
-        top_lp.data_ptr())
-    _lib.call("iw_token_logprobs", C.byref(d), _stream())
+    p = floats.data_ptr()
+    _lib.call("iw_token_logprobs", _LOGP_DESC.pack(
+        logits.data_ptr(), logits.stride(0) if N > 1 else V, _LOGITS[logits.dtype], N, V, scale, p_suppress, p_targets,
+        n_given, top, p, p + 4 * N * n_given, ids.data_ptr(), p + 4 * N * (n_given + 1)), _raw_stream(dev))
     return lp.view(N, n_given), entropy, ids, top_lp.view(N, top)
