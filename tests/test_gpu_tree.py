@@ -1,0 +1,164 @@
+"""TreeDecoder on the GPU: its logits against the model runner's own decoding,
+byte for byte; trees against the paths that they hold; greedy decoding with
+drafts against greedy decoding without."""
+import numpy as np
+import pytest
+import torch
+
+from i_whisper_b200.checkpoint import ModelDims, synthetic_state_dict
+from i_whisper_b200.synthetic import synthetic_mel_batch
+
+pytestmark = pytest.mark.gpu
+
+DIMS = ModelDims(80, 1500, 384, 6, 1, 51865, 448, 384, 6, 2)
+
+
+@pytest.fixture(scope="module")
+def setup():
+    from i_whisper_b200.model import WhisperIntB200
+    sd = synthetic_state_dict(DIMS, 3)
+    mel = torch.from_numpy(synthetic_mel_batch(DIMS.n_mels, [5, 6, 7], float(sd["encoder.input_alpha"][0]))).cuda()
+    model = WhisperIntB200(DIMS, sd)
+    return sd, model, model.encoder(mel).clone()
+
+
+def dense_logits(model, xa, tokens):
+    """[len(tokens), n_vocab]: logits after each token, one token at a time through the runner's dense cache."""
+    ws = model._dec_workspace(1, len(tokens) + 1)
+    ws["tokens"].zero_()
+    ws["state"].zero_()
+    ws["state"][:, 3] = -1
+    ws["pos"].zero_()
+    ws["tk"].fill_(1)
+    ws["step"].fill_(3)
+    model.cross_kv(xa[None].contiguous(), None, ws)
+    t = torch.tensor(tokens, dtype=torch.int64, device="cuda")
+    out = []
+    for i in range(len(tokens)):
+        ws["step"].fill_(3)
+        model._dec_forward(ws, 1, 1, t[i:].data_ptr(), 1, i, graph_mode=False)
+        out.append(ws["logits"][0, :DIMS.n_vocab].clone())
+    return torch.stack(out)
+
+
+def random_tree(rng, n, vocab=51865):
+    return rng.integers(0, vocab, n).tolist(), [-1] + [int(rng.integers(-1, i)) for i in range(1, n)]
+
+
+def test_chains_match_the_dense_decoder(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    rng = np.random.default_rng(0)
+    toks = [rng.integers(0, DIMS.n_vocab, n).tolist() for n in (19, 1, 7)]
+    dec = TreeDecoder(model, xa)
+    got = dec.step(toks, top=3)
+    want = torch.cat([dense_logits(model, xa[b], toks[b]) for b in range(3)])
+    assert torch.equal(got.logits, want)
+    # the scores are those logits'
+    lp = torch.log_softmax(want.double() / model.logit_alpha, 1)
+    assert torch.allclose(got.top_logprobs.double(), torch.gather(lp, 1, got.top_ids), atol=1e-4)
+    # the second part of the context in another pass
+    dec.accept([range(n) for n in (19, 1, 7)])
+    more = [rng.integers(0, DIMS.n_vocab, n).tolist() for n in (2, 30, 0)]
+    got = dec.step(more)
+    want = [dense_logits(model, xa[b], toks[b] + more[b])[len(toks[b]):] for b in range(3) if more[b]]
+    assert torch.equal(got.logits, torch.cat(want))
+
+
+def test_tree_nodes_match_their_paths(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    rng = np.random.default_rng(1)
+    prompts = [rng.integers(0, DIMS.n_vocab, n).tolist() for n in (5, 17, 30)]
+    dec = TreeDecoder(model, xa, page_size=8)
+    dec.step(prompts)
+    dec.accept([range(len(p)) for p in prompts])
+    trees = [random_tree(rng, n) for n in (40, 9, 1)]
+    got = dec.step([t for t, _ in trees], [p for _, p in trees]).logits
+    start, paths = 0, []
+    for b, (t, p) in enumerate(trees):
+        node = int(rng.integers(0, len(t)))
+        path = [node]
+        while p[path[0]] >= 0:
+            path.insert(0, p[path[0]])
+        want = dense_logits(model, xa[b], prompts[b] + [t[i] for i in path])[len(prompts[b]):]
+        assert torch.equal(got[[start + i for i in path]], want)
+        start += len(t)
+        paths.append(path)
+    # accepting a path leaves the cache as decoding it would have
+    dec.accept(paths)
+    nxt = [[11], [12], [13]]
+    got = dec.step(nxt).logits
+    for b, (t, _) in enumerate(trees):
+        assert torch.equal(got[b], dense_logits(model, xa[b], prompts[b] + [t[i] for i in paths[b]] + nxt[b])[-1])
+
+
+def test_greedy_is_the_same_with_any_drafts(setup):
+    from i_whisper_b200 import _lib
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    sot = model.tokens_spec["sot_sequence"]
+    prompts, n = [list(sot), list(sot) + [400, 11], list(sot)[:1]], 24
+    dec = TreeDecoder(model, xa)
+    plain = dec.greedy(prompts, n, lambda b, h: ([], []))
+    assert dec.passes == n - 1 and all(len(o) == n for o in plain)
+    rng = np.random.default_rng(2)
+
+    def oracle_and_noise(b, hist):
+        """The right continuation hidden in a tree of wrong ones (sometimes cut short)."""
+        done = len(hist) - len(prompts[b])
+        right = plain[b][done:done + int(rng.integers(0, 5))]
+        t, p, last = [], [], -1
+        for tok in right:
+            for _ in range(int(rng.integers(0, 3))):
+                t.append(int(rng.integers(0, DIMS.n_vocab)))
+                p.append(int(rng.integers(-1, len(t) - 1)) if len(t) > 1 else -1)
+            t.append(tok)
+            p.append(last)
+            last = len(t) - 1
+        return t, p
+
+    drafted = TreeDecoder(model, xa, page_size=8)
+    assert drafted.greedy(prompts, n, oracle_and_noise) == plain
+    assert drafted.passes < n - 1
+    # the pool holds exactly the contexts' pages
+    used = sum(-(-c // 8) for c in drafted.lens)
+    assert int(drafted.head.item()) == used
+    owned = drafted.table[drafted.table >= 0].tolist() + drafted.free[used:].tolist()
+    assert sorted(owned) == list(range(drafted.free.numel()))
+    assert _lib.device_status(clear=True) == 0
+
+
+def test_zero_point_form(setup):
+    from i_whisper_b200.model import WhisperIntB200
+    from i_whisper_b200.tree import TreeDecoder
+    sd, model, xa = setup
+    unfolded = WhisperIntB200(DIMS, sd, fold_zero_points=False)
+    rs = torch.empty(xa.shape[0] * xa.shape[1], dtype=torch.int32, device="cuda")
+    from i_whisper_b200 import _lib
+    _lib.call("iw_rowsum_i8", xa.data_ptr(), xa.shape[2], rs.numel(), xa.shape[2], rs.data_ptr(),
+              torch.cuda.current_stream().cuda_stream)
+    toks = [[1, 2, 3], [4], [5, 6]]
+    a, b = TreeDecoder(model, xa).step(toks), TreeDecoder(unfolded, xa, rs).step(toks)
+    assert torch.equal(a.logits, b.logits)
+
+
+def test_refusals(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    dec = TreeDecoder(model, xa, pages=4)
+    with pytest.raises(RuntimeError, match="3 lists"):
+        dec.step([[1]])
+    with pytest.raises(RuntimeError, match="no tokens"):
+        dec.step([[], [], []])
+    with pytest.raises(RuntimeError, match="448"):
+        dec.step([[1] * 449, [], []])
+    with pytest.raises(RuntimeError, match="out of cache pages"):
+        dec.step([[1] * 40, [1] * 40, [1]])
+    with pytest.raises(RuntimeError, match="parents"):
+        dec.step([[1], [1], []], [[-1], [], []])
+    dec.step([[1, 2], [], [3]])
+    with pytest.raises(RuntimeError, match="increasing"):
+        dec.accept([[1, 0], [], []])
+    with pytest.raises(RuntimeError, match="features"):
+        TreeDecoder(model, xa[0])
