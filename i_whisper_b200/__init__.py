@@ -9,6 +9,9 @@ Submodules:
   ops         -- ``<op>_cuda`` torch functions with the reference ``_C`` semantics
   model       -- ``WhisperIntB200``: GPU-resident encoder + greedy decoder (the
                  reference logit filters and argmax run on the device)
+  paged       -- ragged batches over a paged INT8 cache: plan, cache write, tree
+                 attention, token log probabilities (also in ``ops``)
+  tree        -- ``TreeDecoder``: drafted token trees verified on a paged cache
   checkpoint  -- ``i-whisper-int`` v1 checkpoint contract and seeded synthetic checkpoints
   frontend    -- log-mel + INT8 input quantisation on the GPU
   synthetic   -- seeded sine + noise audio windows
