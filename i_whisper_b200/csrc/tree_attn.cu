@@ -584,8 +584,8 @@ constexpr int kManyWarps = 4;
 
 template <int D>
 struct Many {
-    static constexpr int kStages = 8;
-    static constexpr int kBytes = 64 * D;  // 64 keys of K, or 32 of K and the same of V
+    static constexpr int kStages = D == 64 ? 16 : 8;
+    static constexpr int kBytes = 64 * D;  // 64 keys of K or V, or 32 of K and the same of V
     static constexpr int kOutLd = D + 4;
     // the sums of P.V take the ring's place once the tiles are done with
     static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * 2 * 4; }
@@ -601,8 +601,8 @@ struct Many {
 // f = d + floor(d/2) - floor(d/16) is exact, and the bits of
 // 2^(7 + xi) * (1 + fr / 2^(fb+1)), f = xi * 2^fb + fr, follow by two integer
 // multiply-adds; its whole part is the probability. Valid for 7 to 14
-// fraction bits, shifts 1 to 9 and rows whose maximum and cut-off lie inside 16
-// bits (so that the clamps of x change nothing).
+// fraction bits and shifts 1 to 9; without CLAMP for rows whose maximum and
+// cut-off lie inside 16 bits, so that the clamps of x change nothing.
 struct FastExp {
     int32_t mult, shift, limit, below, mask, scale, zero, half;
 };
@@ -624,9 +624,17 @@ IW_DEV FastExp fast_exp(const TreeAttnArgs &a) {
 IW_DEV int64_t fast_base(int32_t xm, const FastExp &k) {
     return ((int64_t)(kBias - xm) << k.shift) + ((int64_t)1 << (k.shift - 1));
 }
-IW_DEV uint32_t fast_prob(int32_t acc, int64_t base, const FastExp &k) {
+// CLAMP: for any row. `low` = kBias - 32768 - xm is where x is clamped below; clamped
+// above it is 1 below xm; and the difference of both clamps wraps to 0, the
+// largest probability.
+template <bool CLAMP>
+IW_DEV uint32_t fast_prob(int32_t acc, int64_t base, int32_t low, const FastExp &k) {
     const int64_t t = (int64_t)acc * k.mult + base;
     int32_t d = (int32_t)__funnelshift_r((uint32_t)t, (uint32_t)(t >> 32), k.shift);
+    if (CLAMP) {
+        d = min(max(d, low), kBias - 1);
+        if (d == kBias - 65536) return 128;
+    }
     d = d < k.limit ? k.below : d;
     const float x = __int_as_float(d);
     const float f = __fadd_rn(x, __fadd_rn(__fmaf_rd(x, 0.5f, 6291456.f), -__fmaf_rd(x, 0.0625f, 11796480.f)));
@@ -658,8 +666,8 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     // RT groups of 16 rows side by side, KG sets of warps that share out the tiles:
     // set i takes tiles of 64 keys i, i + KG, ... through SG slots of the ring that
     // are its own (a set has to see every phase of the barriers it waits on)
-    const int lrt = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2), lkg = 2 - lrt, lsg = 3 - lkg;
-    static_assert(kManyWarps == 4 && S == 8, "powers of two above");
+    const int lrt = rows <= 16 ? 0 : (rows <= 32 ? 1 : 2), lkg = 2 - lrt, lsg = (S == 16 ? 4 : 3) - lkg;
+    static_assert(kManyWarps == 4 && (S == 8 || S == 16), "powers of two above");
     const int RT = 1 << lrt, KG = 1 << lkg, SG = 1 << lsg;
     const int first_row = (int)(blockIdx.x >> lr) * 16 * RT, row_step = (int)(gridDim.x >> lr) * 16 * RT;
     if (first_row >= rows) return;
@@ -673,6 +681,10 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     const int first = (tiles * rank) >> lr, mine = ((tiles * (rank + 1)) >> lr) - first;
     cg::cluster_group cl = cg::this_cluster();
     SlabWait slab_wait;
+    // keys few enough that K and V fill the ring once and stay, for the only block of
+    // rows there is: K tile i in slot i, V tile i in slot S/2 + i. (Not at 128 channels,
+    // where the ring would hold 256 keys and the registers are needed elsewhere.)
+    const bool resident = D == 64 && mine <= S / 2 && first_row + row_step >= rows;
 
     if (warp == kManyWarps) {  // the feeder: K tiles, then K and V tiles in turn, for every block of rows
         const int8_t *kbase = a.k + kvh * a.head_stride, *vbase = a.v + kvh * a.head_stride;
@@ -686,33 +698,45 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             if ((uint32_t)pages >= a.n_pages) pages = -1;
         };
         if (TMA) window(0);
-        uint32_t done = 0;  // blocks of rows fed
-        // slot `at` of a set's in this block of rows, filled with the 32 keys of half
-        // tile i and, of the first pass, the next 32, of the second, their V
-        auto put = [&](int set, int at, int i, bool pass2) {
-            const uint32_t count = (mine - set + KG - 1) >> lkg, n = 3 * count * done + (pass2 ? count : 0) + at;
-            const uint32_t slot = (set << lsg) + (n & (SG - 1));
-            if (n >= SG) slab_wait(&empty[slot], ((n >> lsg) - 1) & 1);
+        // a slot filled from half tile i (32 keys): with its K and the next's, its V and
+        // the next's, or its K and its V
+        enum { kKeys, kValues, kBoth };
+        auto fill = [&](uint32_t slot, int i, int what) {
             uint8_t *dst = smem + slot * F::kBytes;
             const int j0 = first * kTile + i * 32;
             if (TMA) {
                 const int w = (i * per) & 31;
                 if (w == 0 && mine * 2 * per > 32) window(i);
-                const int32_t page = __shfl_sync(0xffffffffu, pages, pass2 ? w + (lane & (per - 1)) : w + lane);
+                const int32_t page = __shfl_sync(0xffffffffu, pages, what == kBoth ? w + (lane & (per - 1)) : w + lane);
                 const bool ok = lane < 2 * per && page >= 0;
                 const uint32_t n_box = __popc(__ballot_sync(0xffffffffu, ok));
                 if (lane == 0) mbar_arrive_expect_tx(&full[slot], n_box * box * D);
                 __syncwarp();
-                const bool v = pass2 && lane >= per;
-                const int j = j0 + (v ? lane - per : lane) * box;
+                const bool v = what == kValues || (what == kBoth && lane >= per);
+                const int j = j0 + (what == kBoth && v ? lane - per : lane) * box;
                 if (ok)
                     tma_load_4d(v ? &tmap_v : &tmap_k, &full[slot], dst + lane * box * D, 0, j & ((1 << a.page_log2) - 1), kvh,
                                 page);
             } else {
-                load_rows<D, 32 * D>(a, r, kbase, j0, dst);
-                load_rows<D, 32 * D>(a, r, pass2 ? vbase : kbase, pass2 ? j0 : j0 + 32, dst + 32 * D);
+                load_rows<D, 32 * D>(a, r, what == kValues ? vbase : kbase, j0, dst);
+                load_rows<D, 32 * D>(a, r, what == kKeys ? kbase : vbase, what == kBoth ? j0 : j0 + 32, dst + 32 * D);
                 mbar_arrive_cp_async(&full[slot]);
             }
+        };
+        if (resident) {
+            for (int i = 0; i < mine; ++i) fill(i, 2 * i, kKeys);
+            for (int i = 0; i < mine; ++i) fill(S / 2 + i, 2 * i, kValues);
+            if (ranks > 1) cl.sync(), cl.sync(), cl.sync();
+            __syncthreads();
+            return;
+        }
+        uint32_t done = 0;  // blocks of rows fed
+        // place `at` of a set's slots in this block of rows
+        auto put = [&](int set, int at, int i, bool pass2) {
+            const uint32_t count = (mine - set + KG - 1) >> lkg, n = 3 * count * done + (pass2 ? count : 0) + at;
+            const uint32_t slot = (set << lsg) + (n & (SG - 1));
+            if (n >= SG) slab_wait(&empty[slot], ((n >> lsg) - 1) & 1);
+            fill(slot, i, pass2 ? kBoth : kKeys);
         };
         auto put2 = [&](int i) {  // half tile i of the second pass
             const int tile = i >> 1;
@@ -835,11 +859,13 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
 
         int32_t m0 = INT32_MIN, m1 = INT32_MIN;
         for (int i = kg; i < mine; i += KG, ++n) {
-            arrived(n);
+            if (resident) slab_wait(&full[i], 0);
+            else arrived(n);
+            const uint32_t ks = resident ? ring + i * F::kBytes : tile_at(n);
 #pragma unroll
             for (int h32 = 0; h32 < 2; ++h32) {
                 int32_t c[4][4];
-                raw(c, tile_at(n) + h32 * 32 * D);
+                raw(c, ks + h32 * 32 * D);
                 uint32_t wa, wb;
                 if (!seen((first + i) * kTile + 32 * h32, wa, wb)) {
 #pragma unroll
@@ -856,7 +882,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                     m1 = max(m1, max(c[j][2], c[j][3]));
                 }
             }
-            release(n);
+            if (!resident) release(n);
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
@@ -885,17 +911,27 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             for (int e = 0; e < 8; ++e) o[i][e >> 2][e & 3] = 0;
         uint32_t sum0 = 0, sum1 = 0;
         for (int i = 0; i < 2 * ((mine - kg + KG - 1) >> lkg); ++i, ++n) {
-            const int j0 = (first + kg + (i >> 1) * KG) * kTile + 32 * (i & 1);
+            const int tile = kg + (i >> 1) * KG, j0 = (first + tile) * kTile + 32 * (i & 1);
             uint32_t p[4];
-            arrived(n);
+            if (!resident) arrived(n);
+            const uint32_t half = 32 * (i & 1) * D;
+            const uint32_t ks = resident ? ring + tile * F::kBytes + half : tile_at(n);
+            const uint32_t vs = voff + (resident ? ring + (S / 2 + tile) * F::kBytes + half : ks + 32 * D);
             {
                 int32_t c[4][4];
-                raw(c, tile_at(n));
+                raw(c, ks);
                 if (fast) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) c[j][e] = (int32_t)fast_prob(c[j][e], e < 2 ? base_a : base_b, fx);
+                        for (int e = 0; e < 4; ++e) c[j][e] = (int32_t)fast_prob<false>(c[j][e], e < 2 ? base_a : base_b, 0, fx);
+                } else if (fast_ok) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            c[j][e] = (int32_t)fast_prob<true>(c[j][e], e < 2 ? base_a : base_b,
+                                                               kBias - 32768 - (e < 2 ? xa : xb), fx);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
@@ -925,7 +961,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             }
             sum0 = __dp4a(p[0], 0x01010101u, __dp4a(p[2], 0x01010101u, sum0));
             sum1 = __dp4a(p[1], 0x01010101u, __dp4a(p[3], 0x01010101u, sum1));
-            const uint32_t vs = tile_at(n) + 32 * D + voff;
+            if (resident) slab_wait(&full[S / 2 + tile], 0);
 #pragma unroll
             for (int c = 0; c < D / 16; ++c) {
                 uint32_t v[4];
@@ -933,7 +969,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
                 mma_s8u8(o[c][0], v[0], v[1], v[2], v[3], p[0], p[2]);
                 mma_s8u8(o[c][1], v[0], v[1], v[2], v[3], p[1], p[3]);
             }
-            release(n);
+            if (!resident) release(n);
         }
         // sums over the warps that shared the tiles, then over the cluster
         sum0 += __shfl_xor_sync(0xffffffffu, sum0, 1);
