@@ -98,6 +98,22 @@ struct Row {
     IW_DEV int edge(int t) const { return t < head ? t : (t < head + tail ? t + vecs * kPer : -1); }
 };
 
+// The thread's vectors, U loads in flight at a time.
+template <int kThreads, int U, typename T, typename F>
+IW_DEV void for_vectors(const Row<T> &row, int tid, F f) {
+    int v = tid;
+#pragma unroll 1
+    for (; v + (U - 1) * kThreads < row.vecs; v += U * kThreads) {
+        int4 w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = row.load(v + u * kThreads);
+#pragma unroll
+        for (int u = 0; u < U; ++u) f(v + u * kThreads, w[u]);
+    }
+#pragma unroll 1
+    for (; v < row.vecs; v += kThreads) f(v, row.load(v));
+}
+
 // kPer suppression bits from element i on.
 template <int N>
 IW_DEV uint32_t bits_at(const uint32_t *bits, int i, int V) {
@@ -124,7 +140,7 @@ IW_DEV float max_nan(float a, float b) {
 }
 
 template <typename T, bool SUP, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) == 1 ? 6 : 4)) token_logprobs_kernel(LogprobsArgs a) {
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) == 1 ? 6 : 3)) token_logprobs_kernel(LogprobsArgs a) {
     constexpr bool kBytes = sizeof(T) == 1;
     constexpr int P = Row<T>::kPer, kWarps = kThreads / 32;
     pdl_wait();
@@ -169,12 +185,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
                     }
             }
         };
-        for (int v = tid; v < row.vecs; v += kThreads) {
-            const int4 w = row.load(v);
+        auto vector = [&](int v, const int4 &w) {
             uint32_t sup = 0;
             if (SUP) sup = bits_at<16>(a.suppress, row.first(v), a.V);
             words(w.x, w.y, sup & 255), words(w.z, w.w, sup >> 8);
-        }
+        };
+        for_vectors<kThreads, 4>(row, tid, vector);
         const int e = row.edge(tid);
         const bool extra = e >= 0 && !gone(e);
         if (extra) {
@@ -264,8 +280,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
                 Wm = fmaf(ex, t, Wm);
             }
         };
-        for (int v = tid; v < row.vecs; v += kThreads) {
-            const int4 w = row.load(v);
+        auto vector = [&](int v, const int4 &w) {
             float f[P];
             if constexpr (sizeof(T) == 4) {
                 f[0] = __int_as_float(w.x), f[1] = __int_as_float(w.y), f[2] = __int_as_float(w.z), f[3] = __int_as_float(w.w);
@@ -283,7 +298,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
                 }
             }
             take(f);
-        }
+        };
+        for_vectors<kThreads, 2>(row, tid, vector);
         const int e = row.edge(tid);
         if (e >= 0 && !gone(e)) {
             float f[P];
