@@ -1091,15 +1091,18 @@ static cudaError_t few_rows(const TreeAttnArgs &a, const CacheMaps &m, bool tma,
         if (p.warps < 4) p.warps *= 2;
         else p.ranks *= 2;
     }
-    // fewer rows at a time while the SMs have fewer than 4 warps each: a warp's
-    // time goes by its rows
+    // A request of many rows among others of few takes 8 at a time; a batch of single
+    // tokens has no such request. Fewer at a time too while the SMs have fewer than 4
+    // warps each: a warp's time goes by its rows (7 rows of 12 keys on 6 heads: 16 us
+    // by one warp a head, 10 by one a row)
     const int64_t guess = std::min<int64_t>(kFewRows, mean_rows);
-    while (p.group > 1 && (p.group >= 2 * guess || pairs * p.warps * p.ranks * ((guess + p.group - 1) / p.group) < 4 * num_sms()))
-        p.group /= 2;
+    if (a.N <= a.B)
+        while (p.group >= 2 * guess) p.group /= 2;
+    while (p.group > 1 && pairs * p.warps * p.ranks * ((guess + p.group - 1) / p.group) < 4 * num_sms()) p.group /= 2;
     p.row_blocks = (int)((guess + p.group - 1) / p.group);
     // room for the scores of every slab
     const int64_t per_warp = (keys / Slab<D>::kKeys / p.ranks + p.warps) / p.warps;
-    p.slots = (int)std::min<int64_t>(64, std::max<int64_t>(1, per_warp) * p.group);
+    p.slots = (int)std::min<int64_t>(64, std::max<int64_t>(p.group, per_warp * std::min<int64_t>(p.group, guess)));
     return p.group == 1 ? few_rows_warps<D, 1>(a, m, tma, p, st) : few_rows_warps<D, kFewRows>(a, m, tma, p, st);
 }
 

@@ -69,6 +69,14 @@ def test_plan(ops, B, page, tree):
     assert _check_plan(ops, ctx, new, page, width, 60 * B * 8 // page + 64 * B, 3, N + 5, par, 40 if tree else None) == 0
 
 
+def test_plan_most_requests(ops):
+    from i_whisper_b200 import _lib
+    rng = np.random.default_rng(1)
+    B = _lib.PLAN_MAX_REQUESTS
+    ctx, new = rng.integers(0, 40, B).tolist(), rng.integers(0, 3, B).tolist()
+    assert _check_plan(ops, ctx, new, 8, 6, 2 * B, 0, sum(new) + 1) == 0
+
+
 def test_plan_chain_of_drafts_crosses_mask_words(ops):
     new = [70, 1, 64, 33]
     par = np.concatenate([np.arange(n, dtype=np.int32) - 1 for n in new])
@@ -284,6 +292,71 @@ def test_tree_attention_parameters(ops, mult, shift, fb, av, off, D):
     _check_attn(ops, c, mult, shift, fb, av, off)
 
 
+# (multiplier, shift, frac_bits): rows whose maximum saturates, rows far below 0, shifts on both sides of 9, every
+# number of fraction bits
+MANY_PARAMS = [(118, 8, 13), (255, 3, 13), (255, 1, 14), (255, 0, 12), (0, 5, 13), (70, 31, 13), (70, 9, 13), (90, 10, 13),
+               (255, 2, 7), (30, 4, 8), (90, 6, 9), (90, 6, 10), (90, 5, 11), (120, 6, 12), (64, 6, 15), (90, 6, 16), (90, 6, 1),
+               (90, 6, 6), (1, 9, 7)]
+
+
+@pytest.mark.parametrize("mult,shift,fb", MANY_PARAMS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("low", [False, True])
+def test_tree_attention_parameters_many_rows(ops, mult, shift, fb, D, low):
+    c = _attn_case(fb * 100 + shift, [70, 3, 150], [18, 40, 33], 1, 1, D, 16, True, sd=40)
+    if low:  # every score far below 0
+        c["q"], c["kc"] = np.abs(c["q"].astype(np.int16)).clip(1, 127).astype(np.int8), -np.abs(
+            c["kc"].astype(np.int16)).clip(1, 127).astype(np.int8)
+    _check_attn(ops, c, mult, shift, fb, (88, 5), 16)
+
+
+@pytest.mark.parametrize("ctx,new,Hkv,G,D,page,tree", [
+    ([300], [70], 2, 1, 64, 16, False),            # a chain over several blocks of rows
+    ([500, 20], [30, 64], 1, 4, 64, 128, True),    # pages longer than a tile
+    ([511, 513], [12, 11], 2, 1, 64, 32, True),    # around what stays in shared memory
+    ([260, 700], [33, 20], 1, 2, 128, 8, True),
+    ([90, 600], [20, 31], 1, 2, 128, 4, True),     # pages too short for tensor maps
+    ([77, 5], [17, 40], 2, 1, 64, 2, True),
+    ([3000], [24], 1, 4, 128, 64, True),           # keys split over a cluster
+    ([2500, 31], [16, 1], 1, 1, 64, 16, True),
+    ([0, 0], [64, 40], 1, 1, 64, 16, True),
+    ([10], [300], 1, 1, 128, 16, False),
+    ([1000], [200], 1, 8, 64, 16, False),
+    ([40, 41, 42], [1, 1, 90], 2, 1, 64, 16, True),  # one large tree among single tokens
+    ([40, 41, 42, 3, 4, 5, 6, 7], [1, 1, 50, 1, 1, 1, 1, 1], 2, 1, 64, 16, True),  # the few-rows kernel takes it
+])
+def test_tree_attention_many_rows(ops, ctx, new, Hkv, G, D, page, tree):
+    _check_attn(ops, _attn_case(sum(ctx) + page, ctx, new, Hkv, G, D, page, tree))
+
+
+@pytest.mark.parametrize("fb", [13, 14, 15])
+@pytest.mark.parametrize("new", [[9, 20], [2, 3]])
+def test_tree_attention_extreme_values_by_rows(ops, fb, new):
+    """As test_tree_attention_extreme_values, for either kernel and wide heads."""
+    for D in (64, 128):
+        c = _attn_case(3, [40, 5], new, 1, 1, D, 16)
+        for qv, kv, vv in ((-128, -128, -128), (127, -128, 127), (-128, 127, -128)):
+            c["q"][:], c["kc"][:], c["vc"][:] = qv, kv, vv
+            _check_attn(ops, c, 255, 4, fb, (255, 2))
+        c["q"][:] = 127
+        c["kc"][::2], c["kc"][1::2] = 127, -128
+        for shift in (0, 2, 4, 9):
+            _check_attn(ops, c, 255, shift, fb, (88, 5))
+
+
+def test_tree_attention_holes_many_rows(ops):
+    for D, page in ((64, 16), (128, 64), (64, 128), (64, 4)):
+        c = _attn_case(9, [260, 140, 300], [25, 36, 17], 2, 1, D, page)
+        c["table"][0, 1], c["table"][1, 0], c["table"][2, 2] = -1, 10 ** 6, -7
+        c["ctx"][1] = 5000
+        _check_attn(ops, c)
+
+
+def test_tree_attention_rows_that_see_nothing_many_rows(ops):
+    c = _attn_case(11, [0, 0, 20], [39, 20, 39], 2, 2, 64, 8, empty_rows=True)
+    assert _check_attn(ops, c)[1].count_nonzero() == 0
+
+
 @pytest.mark.parametrize("fb", [13, 15])
 def test_tree_attention_extreme_values(ops, fb):
     """-128 everywhere, alternating extremes, and negative scores only."""
@@ -429,9 +502,10 @@ def _lp_tol(V, x, scale):
     the differences are rounded once; terms more than 100 below the maximum vanish, so the logits that count
     are no larger than the row's maximum plus 100. The entropy weights this by the mean distance from the maximum, at most
     log V plus the entropy's own size. -> [N, 1]"""
-    top = np.where(np.isfinite(x), x, -np.inf).max(1, keepdims=True) * scale
-    low = np.where(np.isfinite(x), x, np.inf).min(1, keepdims=True) * scale
-    big = np.where(np.isfinite(top), np.abs(top) + np.minimum(100.0, top - low), 0.0)
+    some = np.isfinite(x).any(1, keepdims=True)
+    top = np.where(some, np.where(np.isfinite(x), x, -np.inf).max(1, keepdims=True), 0.0) * scale
+    low = np.where(some, np.where(np.isfinite(x), x, np.inf).min(1, keepdims=True), 0.0) * scale
+    big = np.abs(top) + np.minimum(100.0, top - low)
     return 2.0 ** -24 * (V / 128 + 32 + 8 * big) * (1 + np.log(V))
 
 
@@ -578,3 +652,8 @@ def test_logprobs_refusals(ops):
             ops.token_logprobs_cuda(a, **kw)
     lp, ent, ids, top = ops.token_logprobs_cuda(x[:0], top=2)
     assert lp.shape == (0, 0) and ent.shape == (0,) and ids.shape == top.shape == (0, 2)
+
+
+def test_no_wait_ran_out(ops):
+    from i_whisper_b200 import _lib
+    assert _lib.device_status(clear=True) == 0
