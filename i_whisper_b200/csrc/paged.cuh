@@ -59,6 +59,7 @@ struct TreeAttnArgs {
     int32_t frac_bits;
     int32_t av_mult;
     uint32_t av_shift, rsqrt_offset;
+    bool largest_first;  // at most 32 requests, taken by decreasing work
 };
 cudaError_t tree_attention(const TreeAttnArgs &a, cudaStream_t st);
 

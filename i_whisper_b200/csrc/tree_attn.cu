@@ -78,6 +78,26 @@ IW_DEV Request request(const TreeAttnArgs &a, int b) {
     return r;
 }
 
+// The request that block row z serves: of up to 32 long requests the z-th by
+// decreasing work, so that the last blocks to start are not the longest (16
+// requests of 1000 to 8191 keys and 24 to 64 tokens on 4 x 8 heads, the longest
+// given last: 355 us in the given order, 321 so).
+IW_DEV int pick_request(const TreeAttnArgs &a, int z) {
+    if (!a.largest_first) return z;
+    const int lane = threadIdx.x & 31;
+    int64_t work = -1;
+    if (lane < a.B) {
+        const int64_t fresh = max(a.starts[lane + 1] - a.starts[lane], 0);
+        work = fresh ? (max(a.ctx[lane], 0) + fresh) * ((fresh * a.G + 15) / 16) : 0;
+    }
+    int before = 0;
+    for (int j = 0; j < a.B; ++j) {
+        const int64_t other = __shfl_sync(0xffffffffu, work, j);
+        before += other > work || (other == work && j < lane);
+    }
+    return __ffs(__ballot_sync(0xffffffffu, lane < a.B && before == z)) - 1;
+}
+
 // Byte offset of row j of a page within the caches' head.
 IW_DEV uint64_t row_at(const TreeAttnArgs &a, int32_t page, int j) {
     return (uint64_t)(uint32_t)page * a.page_stride + (uint64_t)((uint32_t)j & ((1u << a.page_log2) - 1)) * a.row_stride;
@@ -267,15 +287,15 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
     int32_t *score = scores + warp * slots * kScoreLd, *s_o = scores + W * slots * kScoreLd;
     int32_t *s_sum = s_o + NR * OLD, *s_max = s_sum + NR;
     const int lr = 31 - __clz(ranks);  // a power of two
-    const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+    const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, G = a.G;
     if (lane < S) mbar_init(&bars[lane], TMA ? 1 : 32);
     fence_mbar_init();
     if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     __syncwarp();
     pdl_wait();
     pdl_launch();
-    if (b == a.B - 1) zero_padding(a, kvh, blockIdx.x, gridDim.x);
-    const Request r = request(a, b);
+    if (blockIdx.z == a.B - 1) zero_padding(a, kvh, blockIdx.x, gridDim.x);
+    const Request r = request(a, pick_request(a, blockIdx.z));
     const int rows = r.fresh * G, first_row = (int)(blockIdx.x >> lr) * group, row_step = (int)(gridDim.x >> lr) * group;
     if (first_row >= rows) return;
     const int8_t *kbase = a.k + kvh * a.head_stride, *vbase = a.v + kvh * a.head_stride;
@@ -656,12 +676,12 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S * F::kBytes), *empty = full + S;
     int32_t *s_o = reinterpret_cast<int32_t *>(smem), *s_sum = reinterpret_cast<int32_t *>(empty + S), *s_max = s_sum + 64;
     const int lr = 31 - __clz(ranks);  // a power of two
-    const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, b = blockIdx.z, G = a.G;
+    const int rank = blockIdx.x & (ranks - 1), kvh = blockIdx.y, G = a.G;
     if (TMA && tid == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v);
     pdl_wait();
     pdl_launch();
-    if (b == a.B - 1) zero_padding(a, kvh, blockIdx.x, gridDim.x);
-    const Request r = request(a, b);
+    if (blockIdx.z == a.B - 1) zero_padding(a, kvh, blockIdx.x, gridDim.x);
+    const Request r = request(a, pick_request(a, blockIdx.z));
     const int rows = r.fresh * G;
     // RT groups of 16 rows side by side, KG sets of warps that share out the tiles:
     // set i takes tiles of 64 keys i, i + KG, ... through SG slots of the ring that
@@ -1142,7 +1162,9 @@ static cudaError_t attention(const TreeAttnArgs &a, cudaStream_t st) {
 
 cudaError_t tree_attention(const TreeAttnArgs &a, cudaStream_t st) {
     if (a.B == 0) return cudaMemset2DAsync(a.y, a.ldy, 0, (size_t)a.H * a.D, (size_t)a.N, st);
-    return a.D == 64 ? tree::attention<64>(a, st) : tree::attention<128>(a, st);
+    TreeAttnArgs b = a;
+    b.largest_first = a.B > 1 && a.B <= 32 && ((int64_t)a.width << a.page_log2) > 1024;
+    return a.D == 64 ? tree::attention<64>(b, st) : tree::attention<128>(b, st);
 }
 
 }  // namespace iw
