@@ -6,12 +6,14 @@
 // One block per row reads it once, 16 bytes per thread and load.
 //   Floating types: each thread keeps a running maximum and the sums relative to
 //   it, rescaled when the maximum moves; in units of log 2, so that the
-//   exponential is one instruction. Bound by HBM at 32 bits, by the issue of about
-//   six instructions per element at 16.
+//   exponential is one instruction. Bound by issue at 16 bits, a dozen instructions per
+//   element with suppressed ids: 1031 rows of 100003 bf16 logits, 3 given tokens, 20
+//   alternatives, 74 us, 2.8 TB/s.
 //   int8: there are 256 logits, so the row's histogram says it all: each lane
 //   counts into a column of its own (bank = lane, no conflicts), and the sums
-//   are taken over 256 exact counts. An exponential per element would need more of
-//   its unit than HBM feeds.
+//   are taken over 256 exact counts. Bound by the rate of shared-memory
+//   additions: 4096 rows of 51865 logits, 5 alternatives, 74 us, 2.9 TB/s; an
+//   exponential per element measured 90 us.
 // The most likely tokens: each thread knows its own maximum, so at least
 // `top` elements reach the top-th largest of these; the few elements that do
 // are fetched again (a warp per thread that has some) and ranked among
