@@ -248,14 +248,17 @@ struct SlabWait {
 // once from HBM. Blocks of one to four warps, or a cluster of them, serve one
 // (request, key head) and split its keys; each warp streams slabs of 4 KB
 // through a ring of its own (TMA, no block barrier), K first: scores of the
-// slab's keys by 8 rows by mma.sync with the keys as the 16-row operand, the raw scores kept in
-// shared memory so that K is not read again once the maximum over all
-// blocks is known (exchanged through distributed shared memory; the
+// slab's keys by 8 rows by mma.sync with the keys as the 16-row operand, the raw
+// scores kept in shared memory so that K is not read again once the maximum
+// over all blocks is known (exchanged through distributed shared memory; the
 // requantisation is monotone, so the maximum is taken of raw scores); then V:
 // probabilities, one thread per (row, key), and (P.V)^T by mma.sync with V
 // transposed by ldmatrix. mma.sync and not tcgen05: with at most 8 rows the
 // 128-row tile would be padding, and the tensor pipe is far from its limit at
-// HBM rate; what counts is the instructions per slab.
+// HBM rate; what counts is the instructions per slab. 256 single tokens over 0 to
+// 447 keys, 16 heads of 64: 26 us, 4.7 TB/s; 7 over 4097 to 32700 keys, 20 heads: 64
+// us, 5.6 TB/s (2 slabs per ring; 1 measured 29 and 80 us, 3 26 and 81: more leave
+// room for fewer warps).
 // ---------------------------------------------------------------------------
 constexpr int kFewRows = 8;
 
@@ -588,19 +591,24 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
 
 // ---------------------------------------------------------------------------
 // Many rows per key head (trees, prompts, shared key heads): bound by the
-// arithmetic of the integer softmax and the score products. A block, or a
-// cluster of them that splits the keys, serves one (request, key head); four
-// warps compute, a fifth feeds a ring of 4 KB K and V tiles by TMA (a full
-// and an empty barrier per tile). A warp holds 16 rows: scores by mma.sync, the
-// keys of a tile in such an order that a thread's four probabilities are four
-// consecutive operand bytes of P.V, which therefore never leave registers; V
-// transposed by ldmatrix. The maximum needs all keys before the first
-// probability, so K is read twice (the second time from L2) and its products
-// taken twice: keeping 16 rows of scores would take more shared memory than the
-// K that they come from. Warps share a tile between up to four groups of 16
-// rows; with fewer groups they divide the tiles. tcgen05 would hold scores in
-// tensor memory, from where the softmax has to fetch them, and it wants 128
-// rows, which trees of 64 tokens on one head do not have.
+// latency and issue of the integer softmax and the score products. A block, or
+// a cluster of them that splits the keys, serves up to 64 rows of one (request, key
+// head) at a time; four warps compute, a fifth feeds a ring of K and V slots by
+// TMA (a full and an empty barrier per slot). A warp holds 16 rows: scores by
+// mma.sync, the keys of a tile in such an order that a thread's four
+// probabilities are four consecutive operand bytes of P.V, which therefore never
+// leave registers; (P.V)^T by mma.sync with V transposed by ldmatrix. Warps share a
+// tile between up to four groups of 16 rows; with fewer groups they divide the
+// tiles. The maximum needs all keys before the first probability, so the score
+// products are taken twice and K is read twice, the second time from L2, or not
+// at all where K and V of the request fit the ring.
+// 64 requests with trees of 5 to 32 tokens over 64 to 416 keys, 16 heads of 64:
+// 39 us. 16 requests with trees of 24 to 64 tokens over 1000 to 8191 keys, 32 query
+// and 8 key heads of 128: 295 us, 0.3 of what mma.sync does in 8 bits (1.09 POPS
+// measured). More warps per SM, with fewer registers each or the query
+// operands in shared memory, measured 296 to 310 us. tcgen05 would multiply
+// faster, but hold the scores in tensor memory, from where the softmax has to
+// fetch them, and it wants 128 rows, which trees on one head do not have.
 // ---------------------------------------------------------------------------
 constexpr int kManyWarps = 4;
 

@@ -55,7 +55,7 @@ assert (_PLAN_DESC.size, _ATTN_DESC.size, _LOGP_DESC.size) == tuple(
 
 def _chk1(t, name: str, dtype: torch.dtype, n: int, device: int):
     """A contiguous CUDA tensor [n] of `dtype` on CUDA device `device`."""
-    if t.dtype != dtype or t.shape != (n,) or t.get_device() != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or t.get_device() != device or not t.is_contiguous():
         raise RuntimeError(f"{name} must be a contiguous {dtype} tensor [{n}] on cuda:{device}, got {t.dtype} "
                            f"{tuple(t.shape)} on {t.device}")
 
@@ -111,20 +111,20 @@ def paged_plan_cuda(context_lens, new_lens, block_table, free_pages, free_head, 
             raise RuntimeError("parents need max_new, the most new tokens of a request")
         words = (max_new + 31) // 32
     at = context_lens.device
+    # one allocation for the small outputs: a view is cheaper than an allocation
     slots = torch.empty(max_tokens, dtype=torch.int64, device=at)
-    ints = torch.empty(max_tokens * (2 + words) + B + 3, dtype=torch.int32, device=at)
-    mask, request, position, starts, head, status = ints.split_with_sizes(
-        (max_tokens * words, max_tokens, max_tokens, B + 1, 1, 1))
-    p = ints.data_ptr()
-    p_req = p + 4 * max_tokens * words
+    mask = torch.empty((max_tokens, words), dtype=torch.int32, device=at) if words else None
+    ints = torch.empty(max_tokens * 2 + B + 3, dtype=torch.int32, device=at)
+    request, position, starts, head, status = ints.split_with_sizes((max_tokens, max_tokens, B + 1, 1, 1))
+    p_req = ints.data_ptr()
     p_pos = p_req + 4 * max_tokens
     p_starts = p_pos + 4 * max_tokens
     p_head = p_starts + 4 * (B + 1)
     _lib.call("iw_paged_plan", _PLAN_DESC.pack(
         context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), ld, width, free_pages.data_ptr(), n_free,
         free_head.data_ptr(), page_size, max_tokens, parents.data_ptr() if words else 0, max_new or 0, slots.data_ptr(),
-        p_req, p_pos, p if words else 0, p_starts, p_head, p_head + 4), _raw_stream(dev))
-    return PagedPlan(slots, request, position, starts, head, status, mask.view(max_tokens, words) if words else None)
+        p_req, p_pos, mask.data_ptr() if words else 0, p_starts, p_head, p_head + 4), _raw_stream(dev))
+    return PagedPlan(slots, request, position, starts, head, status, mask)
 
 
 def _cache_checks(k_cache, v_cache, device: int):
@@ -242,11 +242,11 @@ def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, 
     if top < 0 or top > min(V, _lib.LOGPROBS_MAX_TOP):
         raise RuntimeError(f"top must be in [0, min(V, {_lib.LOGPROBS_MAX_TOP})], got {top}")
     at = logits.device
-    floats = torch.empty(N * (n_given + 1 + top), dtype=torch.float32, device=at)
-    lp, entropy, top_lp = floats.split_with_sizes((N * n_given, N, N * top))
-    ids = torch.empty(N, top, dtype=torch.int64, device=at)
-    p = floats.data_ptr()
+    lp = torch.empty((N, n_given), dtype=torch.float32, device=at)
+    entropy = torch.empty(N, dtype=torch.float32, device=at)
+    ids = torch.empty((N, top), dtype=torch.int64, device=at)
+    top_lp = torch.empty((N, top), dtype=torch.float32, device=at)
     _lib.call("iw_token_logprobs", _LOGP_DESC.pack(
         logits.data_ptr(), logits.stride(0) if N > 1 else V, _LOGITS[logits.dtype], N, V, scale, p_suppress, p_targets,
-        n_given, top, p, p + 4 * N * n_given, ids.data_ptr(), p + 4 * N * (n_given + 1)), _raw_stream(dev))
-    return lp.view(N, n_given), entropy, ids, top_lp.view(N, top)
+        n_given, top, lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top_lp.data_ptr()), _raw_stream(dev))
+    return lp, entropy, ids, top_lp
