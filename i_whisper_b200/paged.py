@@ -19,9 +19,15 @@ import torch
 
 from . import _lib
 
-# the current stream's handle without a torch.cuda.Stream object around it
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
-    lambda device: torch.cuda.current_stream(device).cuda_stream)
+# the current stream's handle and the current device without the checks and objects
+# of torch.cuda around them (a CUDA tensor is at hand, so CUDA is initialised)
+if hasattr(torch._C, "_cuda_getCurrentRawStream") and hasattr(torch._C, "_cuda_getDevice"):
+    _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+else:
+    _current_device = torch.cuda.current_device
+
+    def _raw_stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _scalar(t, name: str) -> int:
@@ -63,7 +69,7 @@ def _chk1(t, name: str, dtype: torch.dtype, n: int, device: int):
 def _chk_device(t, name: str) -> int:
     """The index of a CUDA tensor's device, which has to be the current one (the call runs on its stream)."""
     i = t.get_device()
-    if i < 0 or i != torch.cuda.current_device():
+    if i < 0 or i != _current_device():
         raise RuntimeError(f"{name} must be on the current CUDA device, got {t.device}")
     return i
 
@@ -110,11 +116,10 @@ def paged_plan_cuda(context_lens, new_lens, block_table, free_pages, free_head, 
         if max_new is None or max_new < 1:
             raise RuntimeError("parents need max_new, the most new tokens of a request")
         words = (max_new + 31) // 32
-    at = context_lens.device
     # one allocation for the small outputs: a view is cheaper than an allocation
-    slots = torch.empty(max_tokens, dtype=torch.int64, device=at)
-    mask = torch.empty((max_tokens, words), dtype=torch.int32, device=at) if words else None
-    ints = torch.empty(max_tokens * 2 + B + 3, dtype=torch.int32, device=at)
+    slots = new_lens.new_empty(max_tokens, dtype=torch.int64)
+    mask = new_lens.new_empty((max_tokens, words)) if words else None
+    ints = new_lens.new_empty(max_tokens * 2 + B + 3)
     request, position, starts, head, status = ints.split_with_sizes((max_tokens, max_tokens, B + 1, 1, 1))
     p_req = ints.data_ptr()
     p_pos = p_req + 4 * max_tokens
@@ -195,7 +200,7 @@ def tree_attention_cuda(q, k_cache, v_cache, block_table, context_lens, starts, 
             raise RuntimeError("tree_mask must be a contiguous int32 CUDA tensor [N, words]")
         p_mask, words = tree_mask.data_ptr(), tree_mask.shape[1]
     if out is None:
-        out = torch.empty(N, H * D, dtype=torch.int8, device=q.device)
+        out = q.new_empty((N, H * D))
     elif out.dtype != torch.int8 or out.shape != (N, H * D) or out.get_device() != dev or out.stride(1) != 1:
         raise RuntimeError(f"out must be an int8 CUDA tensor [{N}, {H * D}] with contiguous rows")
     _lib.call("iw_tree_attention", _ATTN_DESC.pack(
@@ -241,11 +246,10 @@ def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, 
         p_suppress = suppress_bits.data_ptr()
     if top < 0 or top > min(V, _lib.LOGPROBS_MAX_TOP):
         raise RuntimeError(f"top must be in [0, min(V, {_lib.LOGPROBS_MAX_TOP})], got {top}")
-    at = logits.device
-    lp = torch.empty((N, n_given), dtype=torch.float32, device=at)
-    entropy = torch.empty(N, dtype=torch.float32, device=at)
-    ids = torch.empty((N, top), dtype=torch.int64, device=at)
-    top_lp = torch.empty((N, top), dtype=torch.float32, device=at)
+    lp = logits.new_empty((N, n_given), dtype=torch.float32)
+    entropy = lp.new_empty(N)
+    ids = logits.new_empty((N, top), dtype=torch.int64)
+    top_lp = lp.new_empty((N, top))
     _lib.call("iw_token_logprobs", _LOGP_DESC.pack(
         logits.data_ptr(), logits.stride(0) if N > 1 else V, _LOGITS[logits.dtype], N, V, scale, p_suppress, p_targets,
         n_given, top, lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top_lp.data_ptr()), _raw_stream(dev))

@@ -408,6 +408,15 @@ def test_tree_attention_padding_rows_and_missing_pages(ops):
     assert got[18:].count_nonzero() == 0
 
 
+def test_tree_attention_no_requests(ops):
+    """Every row is padding."""
+    z = lambda *s, dtype=torch.int8: torch.zeros(*s, dtype=dtype, device="cuda")
+    out = torch.full((5, 128), 7, dtype=torch.int8, device="cuda")
+    ops.tree_attention_cuda(z(5, 2, 64), z(3, 2, 16, 64), z(3, 2, 16, 64), z(0, 4, dtype=torch.int32), z(0, dtype=torch.int32),
+                            z(1, dtype=torch.int32), 70, 6, 13, 88, 5, out=out)
+    assert out.count_nonzero() == 0
+
+
 def test_tree_attention_wide_block_table_and_many_requests(ops):
     rng = np.random.default_rng(1)
     ctx, new = rng.integers(0, 90, 300).tolist(), rng.integers(0, 4, 300).tolist()
