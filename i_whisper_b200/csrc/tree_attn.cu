@@ -269,6 +269,8 @@ struct Few {
     static constexpr int kRing = kStages * 4096;
     static constexpr int kScoreLd = Slab<D>::kKeys + 4;  // words per row of a slab's raw scores, padded against bank conflicts
     static constexpr int kOutLd = D + 4;
+    // the sums are read 16 bytes at a time
+    static_assert((kRing + kStages * 8) % 16 == 0 && kScoreLd % 4 == 0 && kOutLd % 4 == 0, "16-byte rows behind the ring");
     static size_t smem(int slots) {
         return 1024 + (size_t)W * (kRing + kStages * 8 + slots * kScoreLd * 4) + (NR * kOutLd + 2 * NR) * 4;
     }
@@ -619,7 +621,7 @@ struct Many {
     static constexpr int kOutLd = D + 4;
     // the sums of P.V take the ring's place once the tiles are done with
     static size_t smem() { return 1024 + kStages * (kBytes + 16) + 64 * 2 * 4; }
-    static_assert(64 * kOutLd * 4 <= kStages * kBytes, "the sums fit the ring");
+    static_assert(64 * kOutLd * 4 <= kStages * kBytes && kOutLd % 4 == 0, "the sums fit the ring, rows of 16 bytes");
 };
 
 // The probability of a score from its raw sum, mostly in the FMA pipe (the ALU
