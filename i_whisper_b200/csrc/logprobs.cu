@@ -8,12 +8,13 @@
 //   it, rescaled when the maximum moves; in units of log 2, so that the
 //   exponential is one instruction. Bound by issue at 16 bits, a dozen instructions per
 //   element with suppressed ids: 1031 rows of 100003 bf16 logits, 3 given tokens, 20
-//   alternatives, 74 us, 2.8 TB/s.
+//   alternatives, 70 us, 3.0 TB/s, and 59 us without suppressed ids.
 //   int8: there are 256 logits, so the row's histogram says it all: each lane
 //   counts into a column of its own (bank = lane, no conflicts), and the sums
 //   are taken over 256 exact counts. Bound by the rate of shared-memory
-//   additions: 4096 rows of 51865 logits, 5 alternatives, 74 us, 2.9 TB/s; an
-//   exponential per element measured 90 us.
+//   additions: 4096 rows of 51865 logits, 5 alternatives, 64 us, 3.3 TB/s (54 without
+//   alternatives, 75 with suppressed ids); an exponential per element measured 16 us
+//   more.
 // The most likely tokens: each thread knows its own maximum, so at least
 // `top` elements reach the top-th largest of these; the few elements that do
 // are fetched again (a warp per thread that has some) and ranked among
@@ -29,8 +30,8 @@ namespace lp {
 
 constexpr int kCandidates = 512;
 // Threads per block where the rows fill the GPU: int8 rows want few, since each
-// block zeroes and sums its histogram once (4096 rows: 78 us with 256, 97 with
-// 512), the others 512 (bf16: 110 us with 256). Fewer rows than SMs leave
+// block zeroes and sums its histogram once (512 measured a quarter slower), the
+// others 512 (256 measured a fifth slower). Fewer rows than SMs leave
 // room for 1024 each.
 template <typename T>
 constexpr int threads_of() { return sizeof(T) == 1 ? 256 : 512; }
@@ -49,6 +50,20 @@ IW_DEV void widen(__nv_bfloat16, uint32_t w, float &lo, float &hi) {
 IW_DEV void widen(__half, uint32_t w, float &lo, float &hi) {
     const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w));
     lo = v.x, hi = v.y;
+}
+
+// The elements of a 16-byte vector.
+template <typename T>
+IW_DEV void unpack(const int4 &w, float (&f)[16 / sizeof(T)]) {
+    const uint32_t q[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 4) f[e] = __uint_as_float(q[e]);
+        else if constexpr (sizeof(T) == 2) widen(T(), q[e], f[2 * e], f[2 * e + 1]);
+        else
+#pragma unroll
+            for (int b = 0; b < 4; ++b) f[4 * e + b] = (float)(int8_t)(q[e] >> (8 * b));
+    }
 }
 
 IW_DEV float exp2_approx(float x) {
@@ -129,7 +144,7 @@ struct Shared {
     uint64_t red64[kThreads / 32];
     uint64_t cand[kCandidates];
     uint16_t owners[kThreads];
-    int n_cand, n_owners;
+    int n_cand, n_owners, n_gone;
     uint32_t bins[256], at_least, threshold;  // int8
     float m, S, W;
 };
@@ -156,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
     auto most = [](float p, float q) { return fmaxf(p, q); };
     auto add = [](float p, float q) { return p + q; };
     const float c = a.scale * 1.4426950408889634f;  // scale / ln 2
-    if (tid == 0) s.n_cand = s.n_owners = 0;
+    if (tid == 0) s.n_cand = s.n_owners = s.n_gone = 0;
 
     float mine = -INFINITY;   // the thread's largest logit
     float m, S, W;            // of the row: maximum (unscaled), sum of 2^t, sum of t 2^t with t = c (x - m)
@@ -168,29 +183,27 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
         const uint32_t column = (uint32_t)__cvta_generic_to_shared(hist) + lane * 4;
         uint32_t even = 0, odd = 0;  // largest x + 128 of the bytes 0, 2 and 1, 3, 16 bits each
         auto count = [&](uint32_t u) { asm volatile("red.shared.add.u32 [%0], 1;" ::"r"(column + u * 128)); };
-        auto words = [&](uint32_t w, uint32_t x, uint32_t sup) {
-            w ^= 0x80808080u, x ^= 0x80808080u;
-            if (!SUP || sup == 0) {
+        int n_gone = 0;
+        auto words = [&](uint32_t w, uint32_t x) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) count(__byte_perm(w, 0, 0x4440 + e));
+            for (int e = 0; e < 4; ++e) count(__byte_perm(w, 0, 0x4440 + e));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) count(__byte_perm(x, 0, 0x4440 + e));
-                even = __vimax3_u16x2(even, w & 0x00ff00ffu, x & 0x00ff00ffu);
-                odd = __vimax3_u16x2(odd, __byte_perm(w, 0, 0x4341), __byte_perm(x, 0, 0x4341));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!((sup >> e) & 1)) {
-                        const uint32_t u = __byte_perm(e < 4 ? w : x, 0, 0x4440 + (e & 3));
-                        count(u);
-                        even = __vimax3_u16x2(even, u, 0);
-                    }
-            }
+            for (int e = 0; e < 4; ++e) count(__byte_perm(x, 0, 0x4440 + e));
+            even = __vimax3_u16x2(even, w & 0x00ff00ffu, x & 0x00ff00ffu);
+            odd = __vimax3_u16x2(odd, __byte_perm(w, 0, 0x4341), __byte_perm(x, 0, 0x4341));
         };
-        auto vector = [&](int v, const int4 &w) {
-            uint32_t sup = 0;
-            if (SUP) sup = bits_at<16>(a.suppress, row.first(v), a.V);
-            words(w.x, w.y, sup & 255), words(w.z, w.w, sup >> 8);
+        auto vector = [&](int v, const int4 &q) {
+            uint32_t w[4] = {(uint32_t)q.x ^ 0x80808080u, (uint32_t)q.y ^ 0x80808080u, (uint32_t)q.z ^ 0x80808080u,
+                             (uint32_t)q.w ^ 0x80808080u};
+            if (SUP) {
+                // suppressed bytes count as the smallest value, and are taken off that count below
+                const uint32_t sup = bits_at<16>(a.suppress, row.first(v), a.V);
+                n_gone += __popc(sup);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // four bits to four bytes
+                    w[e] &= ~((((sup >> (4 * e) & 15) * 0x00204081u) & 0x01010101u) * 255u);
+            }
+            words(w[0], w[1]), words(w[2], w[3]);
         };
         for_vectors<kThreads, 4>(row, tid, vector);
         const int e = row.edge(tid);
@@ -201,6 +214,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
             even = __vimax3_u16x2(even, u, 0);
         }
         mine = (float)(int)max(max(even & 0xffffu, even >> 16), max(odd & 0xffffu, odd >> 16)) - 128.f;
+        if (SUP) {
+            n_gone = __reduce_add_sync(0xffffffffu, n_gone);
+            if (lane == 0) atomicAdd(&s.n_gone, n_gone);
+        }
         __syncthreads();
         {  // a thread per value; its 32 counters in an order free of bank conflicts
             uint32_t cnt = 0;
@@ -210,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
                     const uint4 q = reinterpret_cast<const uint4 *>(hist)[tid * 8 + ((j + lane) & 7)];
                     cnt += q.x + q.y + q.z + q.w;
                 }
+                if (SUP && tid == 0) cnt -= s.n_gone;
                 s.bins[255 - tid] = cnt;  // from the largest value down
             }
         }
@@ -284,13 +302,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
         };
         auto vector = [&](int v, const int4 &w) {
             float f[P];
-            if constexpr (sizeof(T) == 4) {
-                f[0] = __int_as_float(w.x), f[1] = __int_as_float(w.y), f[2] = __int_as_float(w.z), f[3] = __int_as_float(w.w);
-            } else {
-                const uint32_t q[4] = {(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) widen(T(), q[e], f[2 * e], f[2 * e + 1]);
-            }
+            unpack<T>(w, f);
             if (SUP) {
                 const uint32_t sup = bits_at<P>(a.suppress, row.first(v), a.V);
                 if (sup) {
@@ -353,8 +365,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
     if (!slow) {
         if (mine > -INFINITY && order(mine) >= threshold) s.owners[atomicAdd(&s.n_owners, 1)] = (uint16_t)tid;
         __syncthreads();
-        auto offer = [&](int i) {
-            const float v = to_float(row.x[i]);
+        auto offer = [&](int i, float v) {
             if (!(v > -INFINITY) || order(v) < threshold || gone(i)) return;
             const int at = atomicAdd(&s.n_cand, 1);
             if (at < kCandidates) s.cand[at] = key_of(v, i);
@@ -363,10 +374,14 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) ==
         const int owners = s.n_owners;
         for (int k = warp; k < owners; k += kWarps) {
             const int t = s.owners[k];
-            for (int v = t + lane * kThreads; v < row.vecs; v += 32 * kThreads)
-#pragma unroll 1
-                for (int e = 0; e < P; ++e) offer(row.first(v) + e);
-            if (lane == 0 && row.edge(t) >= 0) offer(row.edge(t));
+            for (int v = t + lane * kThreads; v < row.vecs; v += 32 * kThreads) {
+                float f[P];
+                unpack<T>(row.load(v), f);
+#pragma unroll
+                for (int e = 0; e < P; ++e) offer(row.first(v) + e, f[e]);
+            }
+            const int e = row.edge(t);
+            if (lane == 0 && e >= 0) offer(e, to_float(row.x[e]));
         }
         __syncthreads();
         const int found = s.n_cand;
