@@ -633,8 +633,9 @@ struct Many {
 // f = d + floor(d/2) - floor(d/16) is exact, and the bits of
 // 2^(7 + xi) * (1 + fr / 2^(fb+1)), f = xi * 2^fb + fr, follow by two integer
 // multiply-adds; its whole part is the probability. Valid for 7 to 14
-// fraction bits and shifts 1 to 9; without CLAMP for rows whose maximum and
-// cut-off lie inside 16 bits, so that the clamps of x change nothing.
+// fraction bits and shifts 1 to 9; without CLAMP for rows whose maximum lies
+// inside 16 bits and whose cut-off lies above -32768, so that a key clamped from
+// below has no probability either way (a cut-off at -32768 itself has one).
 struct FastExp {
     int32_t mult, shift, limit, below, mask, scale, zero, half;
 };
@@ -936,7 +937,7 @@ __global__ void __launch_bounds__(32 * (kManyWarps + 1), D == 64 ? 3 : 2)
             m1 = cluster_max(cl, s_max + 16 * rt + g + 8, ranks);
         }
         const int32_t xa = (m0 == INT32_MIN ? -32768 : requant(m0)) + 1, xb = (m1 == INT32_MIN ? -32768 : requant(m1)) + 1;
-        auto inside = [&](int32_t xm) { return xm <= 32767 && xm - cut >= -32768; };
+        auto inside = [&](int32_t xm) { return xm <= 32767 && xm - cut > -32768; };
         const int64_t base_a = fast_base(xa, fx), base_b = fast_base(xb, fx);
         const bool fast = __all_sync(0xffffffffu, fast_ok && (ra >= rows || inside(xa)) && (rb >= rows || inside(xb)));
 

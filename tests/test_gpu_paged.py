@@ -310,6 +310,71 @@ def test_tree_attention_parameters_many_rows(ops, mult, shift, fb, D, low):
     _check_attn(ops, c, mult, shift, fb, (88, 5), 16)
 
 
+def _exact_scores(xs, D):
+    """A query and keys [len(xs), D] whose products are the given numbers (|x| below 4 * 127^2)."""
+    xs = np.asarray(xs, np.int64)
+    q = np.full(D, 127, np.int8)
+    q[0] = 1
+    k = np.zeros((len(xs), D), np.int64)
+    rest = np.round(xs / 127).astype(np.int64)
+    k[:, 0] = xs - 127 * rest
+    for d in range(1, 5):
+        k[:, d] = np.clip(rest, -127, 127)
+        rest = rest - k[:, d]
+    assert not rest.any() and np.abs(k).max() <= 127
+    return q, k.astype(np.int8)
+
+
+@pytest.mark.parametrize("best", [-9972, -9973, -9974, -9975])
+@pytest.mark.parametrize("fb", [12, 13, 14])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [20, 2])
+def test_tree_attention_other_keys_at_the_lowest_score(ops, best, fb, D, new):
+    """A row's best score around -9974, every other one clamped to -32768: the clamped difference, -22795, is
+    the last with a probability above 0 at 13 and 14 fraction bits, and the unclamped one has none."""
+    c = _attn_case(5, [70], [new], 1, 1, D, 16, tree=False)
+    q, k = _exact_scores([best, -40000], D)
+    c["q"][:], c["kc"][:] = q, k[1]
+    c["kc"][c["table"][0, 0], 0, 3] = k[0]
+    assert np.abs(_check_attn(ops, c, 64, 6, fb, (255, 0)).cpu().numpy().astype(int)).max() > 0
+
+
+@pytest.mark.parametrize("fb", range(7, 15))
+@pytest.mark.parametrize("rows", [1, 9])  # the few-rows and the many-rows kernel
+def test_tree_attention_every_score_difference(ops, fb, rows):
+    """The short forms of the shift exponential, for every difference of a key's score and the row's best, and
+    beside best and other scores past 16 bits, which are clamped: one request per pair of scores, its two keys in
+    the context. The output channels weigh the two probabilities 0, 2, .. 126 to 127, so that the ones near the
+    balance tell any two probabilities up to the largest ordinary one (95) apart."""
+    D, page = 64, 8
+    step = np.arange(65536)
+    top = np.minimum(step // 2, 32767)  # best - other = step: all of 0 .. 65535
+    every = np.arange(-32768, 32768)
+    pairs = np.concatenate([np.stack([top, top - step], 1),                        # every difference
+                            np.stack([every, np.full(65536, -40000)], 1),          # the other one clamped
+                            np.stack([np.full(65536, 40000), every], 1)])          # the best one clamped
+    q, k = _exact_scores(pairs.reshape(-1), D)
+    x = np.clip(pairs, -32768, 32767)
+    p = R.shift_exp(x, R._i16(x.max(1, keepdims=True) + 1), fb)
+    v = np.stack([-2 * np.arange(D), np.full(D, 127)])
+    inv = np.array([R.fisr(s, 16) for s in range(513)])[p.sum(1)]
+    o = R.rounding_rshift(R._i32((p @ v) * inv[:, None]), 16)
+    o = R.rounding_rshift(R._i32(o * inv[:, None]), 16)
+    want = np.clip(R._i32(o * 255), -127, 127).astype(np.int8)
+    i32 = lambda a: dev(np.asarray(a, np.int32))
+    B = 32768
+    for at in range(0, len(pairs), B):
+        kc = torch.zeros(B, 1, page, D, dtype=torch.int8, device="cuda")
+        vc = torch.zeros_like(kc)
+        kc[:, 0, :2] = dev(k.reshape(-1, 2, D)[at:at + B])
+        vc[:, 0, :2] = dev(v.astype(np.int8))
+        got = ops.tree_attention_cuda(dev(q).expand(B * rows, 1, D), kc, vc, i32(np.arange(B)[:, None]), i32([2] * B),
+                                      i32(np.arange(B + 1) * rows), 64, 6, fb, 255, 0,
+                                      tree_mask=torch.zeros(B * rows, 1, dtype=torch.int32, device="cuda"))
+        got = got.view(B, rows, D).cpu().numpy()
+        assert np.array_equal(got, np.broadcast_to(want[at:at + B, None], got.shape))
+
+
 @pytest.mark.parametrize("ctx,new,Hkv,G,D,page,tree", [
     ([300], [70], 2, 1, 64, 16, False),            # a chain over several blocks of rows
     ([500, 20], [30, 64], 1, 4, 64, 128, True),    # pages longer than a tile
