@@ -654,7 +654,13 @@ class WhisperIntB200:
     def cross_kv(self, xa: torch.Tensor, rs_xa: torch.Tensor, ws) -> None:
         """K/V of every cross-attention layer from the encoder output in one
         GEMM, stored head-major [L, 2, H, B, n_audio_ctx, 64]."""
+        dev = self.tok_emb.device
+        if xa.dtype != torch.int8 or xa.dim() != 3 or xa.device != dev or not xa.is_contiguous():
+            raise RuntimeError(f"xa must be contiguous int8 features [B, n_audio_ctx, n_audio_state] on {dev}")
         B, Ta, d = xa.shape
+        if self.cross_kv_w.wz is not None and (rs_xa is None or rs_xa.dtype != torch.int32 or rs_xa.device != dev
+                                               or rs_xa.numel() != B * Ta or not rs_xa.is_contiguous()):
+            raise RuntimeError(f"rs_xa must be the contiguous int32 row sums of xa, {B * Ta} of them, on {dev}")
         self._gemm(xa, d, B * Ta, self.cross_kv_w, ws["cross"], 0, _lib.IW_GEMM_INT8, rowsum=rs_xa,
                    headmajor=(Ta, B))
 

@@ -44,7 +44,8 @@ class TreeScores(NamedTuple):
 class TreeDecoder:
     """Paged decoding state of a batch of utterances.
 
-    ``xa`` [B, n_audio_ctx, d] int8: the encoder's features (``model.encoder``;
+    ``xa`` [B, n_audio_ctx, d] int8: the encoder's features (``model.encoder``; any
+    strides, so that ``xa[:1].expand(8, -1, -1)`` decodes one utterance eight times;
     ``rs_xa``: their row sums, needed only where the checkpoint's zero points
     are not folded). ``pages`` pages of ``page_size`` tokens are shared by
     the batch (default: enough for every utterance's whole text context)."""
@@ -71,7 +72,7 @@ class TreeDecoder:
         # that divides n_audio_ctx cuts them into pages
         page = Ta & -Ta
         ws = dict(cross=torch.empty(L * 2 * H * B * Ta * 64, dtype=torch.int8, device=dev))
-        model.cross_kv(xa, rs_xa, ws)
+        model.cross_kv(xa.contiguous(), rs_xa, ws)  # which takes its rows one after another
         self.cross = ws["cross"].view(L, 2, H, B * Ta // page, page, 64).permute(0, 1, 3, 2, 4, 5)
         self.cross_table = torch.arange(B * Ta // page, dtype=torch.int32, device=dev).view(B, Ta // page)
         self.cross_ctx = i32(B, Ta)

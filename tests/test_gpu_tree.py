@@ -162,3 +162,28 @@ def test_refusals(setup):
         dec.accept([[1, 0], [], []])
     with pytest.raises(RuntimeError, match="features"):
         TreeDecoder(model, xa[0])
+
+
+def test_features_of_any_strides(setup):
+    """Rows taken out of a batch and one utterance decoded several times, as of contiguous copies."""
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    for some in (xa[::2], xa[1:2].expand(3, -1, -1), xa.flip(0), xa.transpose(1, 2).contiguous().transpose(1, 2)):
+        toks = [[1, 2, 3], [4], [5, 6]][:len(some)]
+        want = [dense_logits(model, x, t) for x, t in zip(some, toks)]
+        assert torch.equal(TreeDecoder(model, some).step(toks).logits, torch.cat(want))
+
+
+def test_features_refusals(setup):
+    from i_whisper_b200.model import WhisperIntB200
+    from i_whisper_b200.tree import TreeDecoder
+    sd, model, xa = setup
+    unfolded = WhisperIntB200(DIMS, sd, fold_zero_points=False)
+    rs = torch.zeros(xa.shape[0] * xa.shape[1], dtype=torch.int32, device="cuda")
+    for m, x, r, match in ((model, xa.cpu(), None, "features"), (unfolded, xa, None, "rs_xa"), (unfolded, xa, rs[1:], "rs_xa"),
+                           (unfolded, xa, rs.long(), "rs_xa"), (unfolded, xa, rs.cpu(), "rs_xa"),
+                           (unfolded, xa, rs.repeat(2)[::2], "rs_xa")):
+        with pytest.raises(RuntimeError, match=match):
+            TreeDecoder(m, x, r)
+    with pytest.raises(RuntimeError, match="contiguous"):  # the runner's own decoding takes no strides
+        model.decode(xa[::2], None, 4)
