@@ -77,6 +77,7 @@ class TreeDecoder:
         self.cross_table = torch.arange(B * Ta // page, dtype=torch.int32, device=dev).view(B, Ta // page)
         self.cross_ctx = i32(B, Ta)
         self.suppress = model.suppress_bits
+        self._plan = None
 
     def step(self, tokens: Sequence[Sequence[int]], parents: Optional[Sequence[Sequence[int]]] = None, top: int = 1,
              targets: Optional[torch.Tensor] = None, suppress: bool = False) -> TreeScores:
@@ -102,10 +103,9 @@ class TreeDecoder:
                 raise RuntimeError("parents must have the lists of tokens")
             up = torch.tensor([p for row in parents for p in row], dtype=torch.int32).to(dev, non_blocking=True)
         new = torch.tensor(n_new, dtype=torch.int32).to(dev, non_blocking=True)
+        self._plan = None  # nothing to accept until this pass is through
         plan = ops.paged_plan_cuda(self.ctx, new, self.table, self.free, self.head, self.page_size, N, parents=up,
                                    max_new=most if up is not None else None)
-        self._granted = [-(-(c + n) // self.page_size) for c, n in zip(self.lens, n_new)]
-        self._plan, self._n_new = plan, n_new
         # pages run out only when the caller gave fewer than the batch can need
         if self.free.numel() < self.B * self.table.shape[1] and plan.status.item() & _lib.PLAN_POOL_EXHAUSTED:
             raise RuntimeError("out of cache pages")
@@ -150,6 +150,8 @@ class TreeDecoder:
         logits = logits[:, :dm.n_vocab]
         scores = ops.token_logprobs_cuda(logits, targets, top=top, scale=1.0 / m.logit_alpha,
                                          suppress_bits=self.suppress if suppress else None)
+        self._granted = [-(-(c + n) // self.page_size) for c, n in zip(self.lens, n_new)]
+        self._plan, self._n_new = plan, n_new
         return TreeScores(logits, *scores, plan)
 
     def accept(self, paths: Sequence[Sequence[int]]) -> None:
@@ -157,6 +159,8 @@ class TreeDecoder:
         last pass (indices into its tokens, from the context downwards): their
         K/V rows are moved together behind the context, and pages that the
         rest had taken go back to the pool."""
+        if self._plan is None:
+            raise RuntimeError("no pass to accept paths of")
         plan, n_new, dev, page = self._plan, self._n_new, self.ctx.device, self.page_size
         src, dst, back = [], [], []
         start = 0

@@ -187,3 +187,25 @@ def test_features_refusals(setup):
             TreeDecoder(m, x, r)
     with pytest.raises(RuntimeError, match="contiguous"):  # the runner's own decoding takes no strides
         model.decode(xa[::2], None, 4)
+
+
+def test_a_refused_pass_leaves_the_pool_as_it_was(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    dec = TreeDecoder(model, xa, pages=4)
+    with pytest.raises(RuntimeError, match="pass"):
+        dec.accept([[], [], []])
+    dec.step([[1, 2, 3], [4], []])
+    dec.accept([[0, 1, 2], [0], []])
+    for refused in (lambda: dec.step([[1] * 40, [1] * 40, [1]]), lambda: dec.step([[1], [1], [1]], top=33)):
+        with pytest.raises(RuntimeError, match="out of cache pages|top"):
+            refused()
+        with pytest.raises(RuntimeError, match="pass"):
+            dec.accept([[], [], []])
+        assert dec.head.item() == 2 and dec.lens == [3, 1, 0]
+    got = dec.step([[5], [], [6] * 20]).logits  # the two pages that are left
+    assert torch.equal(got[0], dense_logits(model, xa[0], [1, 2, 3, 5])[-1])
+    assert torch.equal(got[1:], dense_logits(model, xa[2], [6] * 20))
+    dec.accept([[0], [], [0]])
+    owned = dec.table[:, 0].tolist() + dec.free[3:].tolist()
+    assert dec.head.item() == 3 and sorted(owned) == [0, 1, 2, 3]
