@@ -161,6 +161,8 @@ class TreeDecoder:
         rest had taken go back to the pool."""
         if self._plan is None:
             raise RuntimeError("no pass to accept paths of")
+        if len(paths) != self.B:
+            raise RuntimeError(f"accept needs {self.B} paths, an empty one where nothing is kept")
         plan, n_new, dev, page = self._plan, self._n_new, self.ctx.device, self.page_size
         src, dst, back = [], [], []
         start = 0

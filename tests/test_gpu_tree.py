@@ -209,3 +209,17 @@ def test_a_refused_pass_leaves_the_pool_as_it_was(setup):
     dec.accept([[0], [], [0]])
     owned = dec.table[:, 0].tolist() + dec.free[3:].tolist()
     assert dec.head.item() == 3 and sorted(owned) == [0, 1, 2, 3]
+
+
+def test_accept_takes_a_path_of_every_utterance(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    dec = TreeDecoder(model, xa)
+    dec.step([[1, 2], [4], [3]])
+    for paths in ([[0, 1]], [[0, 1], [0]], [[0, 1], [0], [0], [0]]):
+        with pytest.raises(RuntimeError, match="3 paths"):
+            dec.accept(paths)
+    dec.accept([[0, 1], [0], []])
+    assert dec.lens == [2, 1, 0] and dec.ctx.tolist() == [2, 1, 0]
+    with pytest.raises(RuntimeError, match="pass"):
+        dec.accept([[0, 1], [0], []])
