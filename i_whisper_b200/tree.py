@@ -152,13 +152,17 @@ class TreeDecoder:
                                          suppress_bits=self.suppress if suppress else None)
         self._granted = [-(-(c + n) // self.page_size) for c, n in zip(self.lens, n_new)]
         self._plan, self._n_new = plan, n_new
+        # what each token follows, by the plan's rule: no earlier token counts as the context
+        self._up = [[p if 0 <= p < i else -1 for i, p in enumerate(row)]
+                    for row in ([range(-1, n - 1) for n in n_new] if parents is None else parents)]
         return TreeScores(logits, *scores, plan)
 
     def accept(self, paths: Sequence[Sequence[int]]) -> None:
         """Advance each utterance's context by the nodes ``paths[b]`` of the
-        last pass (indices into its tokens, from the context downwards): their
-        K/V rows are moved together behind the context, and pages that the
-        rest had taken go back to the pool."""
+        last pass (indices into its tokens, the first a child of the context,
+        each the parent of the next: other nodes' K/V rows were computed under
+        another history): their K/V rows are moved together behind the context,
+        and pages that the rest had taken go back to the pool."""
         if self._plan is None:
             raise RuntimeError("no pass to accept paths of")
         if len(paths) != self.B:
@@ -169,6 +173,8 @@ class TreeDecoder:
         for b, path in enumerate(paths):
             if any(not 0 <= i < n_new[b] for i in path) or any(i >= j for i, j in zip(path, path[1:])):
                 raise RuntimeError("a path must be increasing indices of the utterance's new tokens")
+            if [self._up[b][i] for i in path] != [-1, *path][:len(path)]:
+                raise RuntimeError("a path must be a branch of the utterance's tree from the context downwards")
             for k, i in enumerate(path):
                 if i != k:
                     src.append(start + i)

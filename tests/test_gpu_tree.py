@@ -223,3 +223,24 @@ def test_accept_takes_a_path_of_every_utterance(setup):
     assert dec.lens == [2, 1, 0] and dec.ctx.tolist() == [2, 1, 0]
     with pytest.raises(RuntimeError, match="pass"):
         dec.accept([[0, 1], [0], []])
+
+
+def test_accept_takes_only_branches(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    dec = TreeDecoder(model, xa)
+    # 0 and 1 follow the context, 2 and 3 follow 0, 4 follows 1; 5's parent is no earlier token
+    dec.step([[1, 2, 3, 4, 5, 6], [1, 2, 3], []], [[-1, -1, 0, 0, 1, 7], [-1, 0, 1], []])
+    for paths in ([[0, 1], [], []], [[2], [], []], [[0, 2, 3], [], []], [[0, 4], [], []], [[0, 5], [], []],
+                  [[], [1], []], [[], [0, 2], []]):
+        with pytest.raises(RuntimeError, match="branch"):
+            dec.accept(paths)
+    assert dec.lens == [0, 0, 0]
+    dec.accept([[5], [0, 1], []])
+    assert dec.lens == [1, 2, 0]
+    dec.step([[1, 2, 3], [1], []])  # chains
+    for paths in ([[1, 2], [], []], [[0, 2], [], []]):
+        with pytest.raises(RuntimeError, match="branch"):
+            dec.accept(paths)
+    dec.accept([[0, 1], [0], []])
+    assert dec.lens == [3, 3, 0]
