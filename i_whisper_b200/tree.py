@@ -93,10 +93,13 @@ class TreeDecoder:
         N, most = sum(n_new), max(n_new)
         if N == 0:
             raise RuntimeError("no tokens")
+        ids = [t for row in tokens for t in row]
+        if min(ids) < 0 or max(ids) >= dm.n_vocab:
+            raise RuntimeError(f"token ids must be in [0, {dm.n_vocab})")
         if any(c + n > dm.n_text_ctx for c, n in zip(self.lens, n_new)):
             raise RuntimeError(f"more than {dm.n_text_ctx} text tokens")
         dev = self.ctx.device
-        flat = torch.tensor([t for row in tokens for t in row], dtype=torch.int64).to(dev, non_blocking=True)
+        flat = torch.tensor(ids, dtype=torch.int64).to(dev, non_blocking=True)
         up = None
         if parents is not None:
             if [len(p) for p in parents] != n_new:

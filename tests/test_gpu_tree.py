@@ -244,3 +244,16 @@ def test_accept_takes_only_branches(setup):
             dec.accept(paths)
     dec.accept([[0, 1], [0], []])
     assert dec.lens == [3, 3, 0]
+
+
+def test_token_ids_outside_the_vocabulary(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    dec = TreeDecoder(model, xa)
+    for bad in (-1, DIMS.n_vocab, 2 ** 40):
+        with pytest.raises(RuntimeError, match="token ids"):
+            dec.step([[1, 2], [], [3, bad]])
+        with pytest.raises(RuntimeError, match="token ids"):
+            dec.step([[1, bad], [], [3]], [[-1, 0], [], [-1]])
+    last = DIMS.n_vocab - 1
+    assert torch.equal(dec.step([[0, last], [], []]).logits, dense_logits(model, xa[0], [0, last]))
