@@ -210,6 +210,8 @@ class TreeDecoder:
         the new tokens, the same whatever is drafted; good drafts take
         fewer passes (``self.passes``)."""
         hist = [list(p) for p in prompts]
+        if not all(hist):
+            raise RuntimeError("greedy needs a prompt of at least one token for every utterance")
         out: List[List[int]] = [[] for _ in prompts]
         self.passes = 0
         first = self.step(hist, suppress=suppress)

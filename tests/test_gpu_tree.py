@@ -257,3 +257,11 @@ def test_token_ids_outside_the_vocabulary(setup):
             dec.step([[1, bad], [], [3]], [[-1, 0], [], [-1]])
     last = DIMS.n_vocab - 1
     assert torch.equal(dec.step([[0, last], [], []]).logits, dense_logits(model, xa[0], [0, last]))
+
+
+def test_greedy_needs_prompts(setup):
+    from i_whisper_b200.tree import TreeDecoder
+    _, model, xa = setup
+    for prompts in ([[], [1], [2]], [[1], [], [2]], [[], [], []]):
+        with pytest.raises(RuntimeError, match="prompt"):
+            TreeDecoder(model, xa).greedy(prompts, 4, lambda b, h: ([], []))
