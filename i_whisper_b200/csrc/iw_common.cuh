@@ -187,7 +187,9 @@ struct SmemLimit {
 
 template <typename... KArgs>
 inline cudaError_t raise_smem_limit(void (*kernel)(KArgs...), size_t bytes, SmemLimit &lim) {
-    if (bytes <= 48 * 1024) return cudaSuccess;  // the default limit
+    // the default limit, 48 KB, is for the kernel's own __shared__ variables too,
+    // which take at most 33 KB here
+    if (bytes <= 15 * 1024) return cudaSuccess;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;

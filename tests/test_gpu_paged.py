@@ -1,6 +1,10 @@
 """The paged, tree-drafted decoding operators on the GPU against plain 64-bit
 implementations (tests/paged_reference.py). Integer outputs are compared bit
 for bit; the tolerance of the log probabilities is derived in `_lp_tol`."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -75,6 +79,23 @@ def test_plan_most_requests(ops):
     B = _lib.PLAN_MAX_REQUESTS
     ctx, new = rng.integers(0, 40, B).tolist(), rng.integers(0, 3, B).tolist()
     assert _check_plan(ops, ctx, new, 8, 6, 2 * B, 0, sum(new) + 1) == 0
+
+
+def test_plan_first_call_around_the_default_shared_memory():
+    """Request counts whose two sums alone fit the default 48 KB of shared memory, but not beside the kernel's own
+    variables, as the first call of a process (later calls would find the limit raised)."""
+    code = """
+import torch
+from i_whisper_b200 import ops
+for B in (6125, 6126, 6143, 6144):
+    one = torch.ones(B, dtype=torch.int32, device="cuda")
+    p = ops.paged_plan_cuda(one, one, torch.zeros(B, 1, dtype=torch.int32, device="cuda"), one[:1], one[:1] * 0, 16, B)
+    assert p.starts.tolist() == list(range(B + 1)) and p.slots.tolist() == [1] * B and p.status.item() == 0
+print("ok")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stdout + run.stderr
 
 
 def test_plan_chain_of_drafts_crosses_mask_words(ops):
