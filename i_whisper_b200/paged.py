@@ -59,6 +59,14 @@ assert (_PLAN_DESC.size, _ATTN_DESC.size, _LOGP_DESC.size) == tuple(
     ctypes.sizeof(d) for d in (_lib.PagedPlanDesc, _lib.TreeAttnDesc, _lib.TokenLogprobsDesc))
 
 
+def _call(name: str, desc: struct.Struct, device: int, *args) -> None:
+    try:
+        packed = desc.pack(*args)
+    except (struct.error, OverflowError) as e:  # a number that its C field does not hold
+        raise RuntimeError(f"{name}: argument out of range: {e}") from None
+    _lib.call(name, packed, _raw_stream(device))
+
+
 def _chk1(t, name: str, dtype: torch.dtype, n: int, device: int):
     """A contiguous CUDA tensor [n] of `dtype` on CUDA device `device`."""
     if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or t.get_device() != device or not t.is_contiguous():
@@ -125,10 +133,10 @@ def paged_plan_cuda(context_lens, new_lens, block_table, free_pages, free_head, 
     p_pos = p_req + 4 * max_tokens
     p_starts = p_pos + 4 * max_tokens
     p_head = p_starts + 4 * (B + 1)
-    _lib.call("iw_paged_plan", _PLAN_DESC.pack(
-        context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), ld, width, free_pages.data_ptr(), n_free,
-        free_head.data_ptr(), page_size, max_tokens, parents.data_ptr() if words else 0, max_new or 0, slots.data_ptr(),
-        p_req, p_pos, mask.data_ptr() if words else 0, p_starts, p_head, p_head + 4), _raw_stream(dev))
+    _call("iw_paged_plan", _PLAN_DESC, dev, context_lens.data_ptr(), new_lens.data_ptr(), B, block_table.data_ptr(), ld,
+          width, free_pages.data_ptr(), n_free, free_head.data_ptr(), page_size, max_tokens,
+          parents.data_ptr() if words else 0, max_new or 0, slots.data_ptr(), p_req, p_pos,
+          mask.data_ptr() if words else 0, p_starts, p_head, p_head + 4)
     return PagedPlan(slots, request, position, starts, head, status, mask)
 
 
@@ -203,12 +211,11 @@ def tree_attention_cuda(q, k_cache, v_cache, block_table, context_lens, starts, 
         out = q.new_empty((N, H * D))
     elif out.dtype != torch.int8 or out.shape != (N, H * D) or out.get_device() != dev or out.stride(1) != 1:
         raise RuntimeError(f"out must be an int8 CUDA tensor [{N}, {H * D}] with contiguous rows")
-    _lib.call("iw_tree_attention", _ATTN_DESC.pack(
-        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
-        st[0], st[1], st[2], P, page, block_table.data_ptr(), ld, width, context_lens.data_ptr(), starts.data_ptr(),
-        p_mask, words, B, N, H, Hkv, D, _scalar(qk_multiplier, "qk_multiplier"), _scalar(qk_shift, "qk_shift"),
-        _scalar(frac_bits, "frac_bits"), _scalar(av_multiplier, "av_multiplier"), _scalar(av_shift, "av_shift"),
-        rsqrt_offset), _raw_stream(dev))
+    _call("iw_tree_attention", _ATTN_DESC, dev, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0),
+          k_cache.data_ptr(), v_cache.data_ptr(), st[0], st[1], st[2], P, page, block_table.data_ptr(), ld, width,
+          context_lens.data_ptr(), starts.data_ptr(), p_mask, words, B, N, H, Hkv, D,
+          _scalar(qk_multiplier, "qk_multiplier"), _scalar(qk_shift, "qk_shift"), _scalar(frac_bits, "frac_bits"),
+          _scalar(av_multiplier, "av_multiplier"), _scalar(av_shift, "av_shift"), rsqrt_offset)
     return out
 
 
@@ -250,7 +257,7 @@ def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, 
     entropy = lp.new_empty(N)
     ids = logits.new_empty((N, top), dtype=torch.int64)
     top_lp = lp.new_empty((N, top))
-    _lib.call("iw_token_logprobs", _LOGP_DESC.pack(
-        logits.data_ptr(), logits.stride(0) if N > 1 else V, _LOGITS[logits.dtype], N, V, scale, p_suppress, p_targets,
-        n_given, top, lp.data_ptr(), entropy.data_ptr(), ids.data_ptr(), top_lp.data_ptr()), _raw_stream(dev))
+    _call("iw_token_logprobs", _LOGP_DESC, dev, logits.data_ptr(), logits.stride(0) if N > 1 else V,
+          _LOGITS[logits.dtype], N, V, scale, p_suppress, p_targets, n_given, top, lp.data_ptr(), entropy.data_ptr(),
+          ids.data_ptr(), top_lp.data_ptr())
     return lp, entropy, ids, top_lp

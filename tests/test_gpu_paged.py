@@ -749,6 +749,25 @@ def test_logprobs_refusals(ops):
     assert lp.shape == (0, 0) and ent.shape == (0,) and ids.shape == top.shape == (0, 2)
 
 
+def test_numbers_out_of_range_are_refused_like_other_arguments(ops):
+    z = lambda *s, dtype=torch.int8: torch.zeros(*s, dtype=dtype, device="cuda")
+    i = lambda *s: z(*s, dtype=torch.int32)
+    kc = z(3, 2, 16, 64)
+    good = [70, 6, 13, 88, 5]
+    for at, bad in ((0, 256), (0, -1), (1, 128), (2, 2 ** 31), (3, 300), (4, -129)):
+        args = list(good)
+        args[at] = bad
+        with pytest.raises(RuntimeError, match="iw_tree_attention"):
+            ops.tree_attention_cuda(z(4, 2, 64), kc, kc, i(1, 3), i(1), i(2), *args)
+    with pytest.raises(RuntimeError, match="iw_tree_attention"):
+        ops.tree_attention_cuda(z(4, 2, 64), kc, kc, i(1, 3), i(1), i(2), *good, rsqrt_offset=2 ** 40)
+    for scale in (1e39, "1"):
+        with pytest.raises(RuntimeError, match="iw_token_logprobs"):
+            ops.token_logprobs_cuda(z(3, 50), scale=scale)
+    with pytest.raises(RuntimeError, match="iw_paged_plan"):
+        ops.paged_plan_cuda(i(2), i(2), i(2, 4), i(1), i(1), 16.0, 2)
+
+
 def test_no_wait_ran_out(ops):
     from i_whisper_b200 import _lib
     assert _lib.device_status(clear=True) == 0
