@@ -5,6 +5,7 @@
 // negative code and records a message for iw_last_error().
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -723,6 +724,20 @@ static int page_log2(int64_t page_size) {
     return -1;
 }
 
+// Whether the rows of a paged cache, `bytes` each, lie apart from one another:
+// in the order of their strides, each axis steps past all that the ones below span.
+static bool rows_apart(int64_t bytes, const int64_t (&sizes)[3], const int64_t (&strides)[3]) {
+    int at[3] = {0, 1, 2};
+    std::sort(at, at + 3, [&](int x, int y) { return strides[x] < strides[y]; });
+    __int128 span = bytes;
+    for (int i : at) {
+        if (sizes[i] <= 1) continue;
+        if (strides[i] < span) return false;
+        span += (__int128)strides[i] * (sizes[i] - 1);
+    }
+    return true;
+}
+
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int iw_paged_plan(const iw_paged_plan_desc *d, void *stream) {
@@ -765,6 +780,8 @@ int iw_paged_kv_write(const int8_t *k, int64_t ldk, int64_t k_hs, const int8_t *
     if (((D | ldk | k_hs | ldv | v_hs | page_stride | head_stride | row_stride) & 15) || !aligned16(k) || !aligned16(v) ||
         !aligned16(k_cache) || !aligned16(v_cache))
         return fail(IW_EINVAL, "iw_paged_kv_write: rows must be 16-byte aligned");
+    if (!rows_apart(D, {n_pages, H, page_size}, {page_stride, head_stride, row_stride}))
+        return fail(IW_EINVAL, "iw_paged_kv_write: the caches' rows must not overlap");
     iw::KvWriteArgs a;
     a.k = k; a.v = v; a.ldk = ldk; a.k_hs = k_hs; a.ldv = ldv; a.v_hs = v_hs; a.slots = slots;
     a.k_cache = k_cache; a.v_cache = v_cache;
@@ -796,6 +813,7 @@ int iw_tree_attention(const iw_tree_attn_desc *d, void *stream) {
     if (((d->ldq | d->q_hs | d->ldy | d->page_stride | d->head_stride | d->row_stride) & 15) || !aligned16(d->q) ||
         !aligned16(d->y) || !aligned16(d->k_cache) || !aligned16(d->v_cache))
         return fail(IW_EINVAL, "iw_tree_attention: rows must be 16-byte aligned");
+    if (d->N > 1 && d->ldy < d->H * d->D) return fail(IW_EINVAL, "iw_tree_attention: output rows must not overlap");
     if (d->page_stride < 0 || d->row_stride < 0 || d->page_stride > INT32_MAX || d->row_stride > INT32_MAX)
         return fail(IW_EINVAL, "iw_tree_attention: page and row strides must be below 2^31 bytes");
     iw::TreeAttnArgs a;

@@ -484,7 +484,8 @@ int iw_paged_plan(const iw_paged_plan_desc *d, void *stream);
  * caches; a page's element (h, r, d) is at page*page_stride + h*head_stride +
  * r*row_stride + d, the same in both. Rows whose slot is negative or not
  * below n_pages*page_size are skipped. D and all strides are multiples of 16
- * bytes, pointers 16-byte aligned. Two rows with one slot leave either. */
+ * bytes, pointers 16-byte aligned; the axes of the caches may be in any order, but
+ * their rows must not overlap. Two rows with one slot leave either. */
 int iw_paged_kv_write(const int8_t *k, int64_t ldk, int64_t k_hs, const int8_t *v, int64_t ldv, int64_t v_hs,
                       const int64_t *slots, int8_t *k_cache, int8_t *v_cache, int64_t page_stride,
                       int64_t head_stride, int64_t row_stride, int64_t n_pages, int64_t page_size, int64_t N,
@@ -492,7 +493,7 @@ int iw_paged_kv_write(const int8_t *k, int64_t ldk, int64_t k_hs, const int8_t *
 
 typedef struct iw_tree_attn_desc {
     const int8_t *q; int64_t ldq, q_hs;  /* [N, H, D]: element q[n*ldq + h*q_hs + d] */
-    int8_t *y; int64_t ldy;              /* [N, H*D]                                 */
+    int8_t *y; int64_t ldy;              /* [N, H*D], rows apart                     */
     const int8_t *k_cache, *v_cache;     /* as in iw_paged_kv_write, Hkv heads       */
     int64_t page_stride, head_stride, row_stride, n_pages, page_size;
     const int32_t *block_table; int64_t table_ld, table_width;

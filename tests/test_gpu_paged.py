@@ -768,6 +768,27 @@ def test_numbers_out_of_range_are_refused_like_other_arguments(ops):
         ops.paged_plan_cuda(i(2), i(2), i(2, 4), i(1), i(1), 16.0, 2)
 
 
+def test_outputs_that_overlap_are_refused(ops):
+    z = lambda *s, dtype=torch.int8: torch.zeros(*s, dtype=dtype, device="cuda")
+    i = lambda *s: z(*s, dtype=torch.int32)
+    kc, k, slots = z(3, 2, 16, 64), z(4, 2, 64), z(4, dtype=torch.int64)
+    for cache in (kc[:1].expand(3, -1, -1, -1), kc[:, :1].expand(-1, 2, -1, -1), kc[:, :, :1].expand(-1, -1, 16, -1),
+                  kc.view(-1).as_strided((3, 2, 16, 64), (1024, 1024, 64, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.paged_kv_write_cuda(k, k, slots, cache, cache)
+    args = (k, kc, kc, i(1, 3), i(1), i(2), 70, 6, 13, 88, 5)
+    for out in (z(1, 128).expand(4, -1), z(1024).as_strided((4, 128), (64, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.tree_attention_cuda(*args, out=out)
+    # one page, head or row: its stride says nothing; caches that lie between one another's rows are apart
+    both = z(3, 2, 2, 16, 64)
+    ops.paged_kv_write_cuda(k, k, slots, both[:, 0], both[:, 1])
+    for cache in (kc[:1], kc[:, :, :1]):
+        ops.paged_kv_write_cuda(k, k, slots, cache, cache)
+    ops.paged_kv_write_cuda(k[:, :1], k[:, :1], slots, kc[:, :1], kc[:, :1])
+    ops.tree_attention_cuda(k[:1], *args[1:], out=z(1, 128).as_strided((1, 128), (0, 1)))
+
+
 def test_no_wait_ran_out(ops):
     from i_whisper_b200 import _lib
     assert _lib.device_status(clear=True) == 0

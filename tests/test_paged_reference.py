@@ -115,3 +115,17 @@ def test_token_logprobs_refusals():
         (dict(top=33), "top"), (dict(top=5, V=4), "top"), (dict(scale=0.0), "scale"), (dict(scale=float("inf")), "scale"),
         (dict(C=1), "null array"), (dict(top=1), "null array"), (dict(dtype=3, logits=FAKE + 2), "aligned")])
     assert _lib.LIB.iw_token_logprobs(C.byref(_lib.TokenLogprobsDesc(**{**good, "N": 0})), None) == _lib.IW_OK
+
+
+def test_outputs_that_overlap_are_refused():
+    """Rows of one output that share memory would be written by several blocks at once."""
+    attn = dict(q=FAKE, ldq=256, q_hs=64, y=FAKE, ldy=256, k_cache=FAKE, v_cache=FAKE, page_stride=4096, head_stride=1024,
+                row_stride=64, n_pages=8, page_size=16, block_table=FAKE, table_ld=4, table_width=4, context_lens=FAKE,
+                starts=FAKE, B=2, N=5, H=4, Hkv=4, D=64, frac_bits=13, rsqrt_offset=16)
+    _reject("iw_tree_attention", _lib.TreeAttnDesc, attn, [(dict(ldy=n), "overlap") for n in (0, 64, 240)])
+    # page_stride, head_stride, row_stride of [8, 4, 16, 64] caches
+    for strides in ((0, 1024, 64), (4096, 0, 64), (4096, 1024, 0), (4096, 1024, 48), (4080, 1024, 64), (4096, 1008, 64),
+                    (64, 512, 512), (2 ** 62, 1024, 32), (1024, 4096, 64)):
+        args = [FAKE, 256, 64, FAKE, 256, 64, FAKE, FAKE, FAKE, *strides, 8, 16, 3, 4, 64, None]
+        with pytest.raises(RuntimeError, match="overlap"):
+            _lib.call("iw_paged_kv_write", *args)
