@@ -222,6 +222,18 @@ def tree_attention_cuda(q, k_cache, v_cache, block_table, context_lens, starts, 
 _LOGITS = {torch.int8: 0, torch.float16: 1, torch.bfloat16: 2, torch.float32: 3}
 
 
+class _Ungraded(torch.autograd.Function):
+    """The scores of logits that ask for a gradient: asking them for it is an error."""
+
+    @staticmethod
+    def forward(ctx, logits, *args):
+        return token_logprobs_cuda(logits, *args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("token_logprobs_cuda has no gradient: it is for inference")
+
+
 def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, suppress_bits=None):
     """Log probabilities of given tokens under softmax(scale * logits).
 
@@ -232,7 +244,11 @@ def token_logprobs_cuda(logits, targets=None, top: int = 0, scale: float = 1.0, 
     Returns (logprobs float32 [N, C], entropy float32 [N], top_ids int64
     [N, top], top_logprobs float32 [N, top]); equal logits are ordered by id,
     and an alternative that does not exist (fewer tokens than ``top`` with a
-    logit above -inf) has id -1 and -inf. A row with a NaN or +inf gives NaN."""
+    logit above -inf) has id -1 and -inf. A row with a NaN or +inf gives NaN.
+    For inference: there is no gradient, and a backward pass through the
+    scores of logits that ask for one raises."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Ungraded.apply(logits, targets, top, scale, suppress_bits)
     dev = _chk_device(logits, "logits")
     if logits.dtype not in _LOGITS:
         raise RuntimeError(f"logits must be int8, float16, bfloat16 or float32, got {logits.dtype}")

@@ -789,6 +789,23 @@ def test_outputs_that_overlap_are_refused(ops):
     ops.tree_attention_cuda(k[:1], *args[1:], out=z(1, 128).as_strided((1, 128), (0, 1)))
 
 
+@pytest.mark.parametrize("kind", ["float16", "bfloat16", "float32"])
+def test_logprobs_gradients_are_refused(ops, kind):
+    """Logits that ask for a gradient give the same scores, and an error where it would be lost."""
+    x = _logits(np.random.default_rng(3), kind, 4, 300).clone()
+    t = torch.tensor([[1], [2], [3], [-1]], device="cuda")
+    want = ops.token_logprobs_cuda(x, t, 3)
+    x.requires_grad_()
+    got = ops.token_logprobs_cuda(x, t, 3)
+    assert all(torch.equal(g.detach(), w) for g, w in zip(got, want))
+    for g in (got[0], got[1], got[3]):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            g.sum().backward(retain_graph=True)
+    assert not got[2].requires_grad
+    with torch.no_grad():
+        assert not any(g.requires_grad for g in ops.token_logprobs_cuda(x, t, 3))
+
+
 def test_no_wait_ran_out(ops):
     from i_whisper_b200 import _lib
     assert _lib.device_status(clear=True) == 0
