@@ -806,6 +806,67 @@ def test_logprobs_gradients_are_refused(ops, kind):
         assert not any(g.requires_grad for g in ops.token_logprobs_cuda(x, t, 3))
 
 
+# Small batches leave each block one row at a time; with enough (request, key head) pairs the few-rows kernel takes
+# eight rows at a time, by 1, 2 or 4 warps a pair and by clusters (the block table's width decides)
+def _many_pairs(seed, B, most, G, width_keys, page, long=()):
+    """Contexts, new-token counts (at most 8 / G on average) and the spare columns that make the block table
+    `width_keys` keys wide; `long` requests come first."""
+    rng = np.random.default_rng(seed)
+    new = rng.integers(1, 8 // G + 1, B)
+    ctx = rng.integers(0, most + 1, B)
+    ctx[1::7], new[2::9] = 0, 0
+    for i, (c, n) in enumerate(long):
+        ctx[i], new[i] = c, n
+    cols = -(-int((ctx + new).max()) // page)
+    return ctx.tolist(), new.tolist(), max(width_keys // page - cols, 0)
+
+
+@pytest.mark.parametrize("B,Hkv,G,most,width_keys,long", [
+    (150, 4, 1, 50, 64, ()),                          # a warp per pair
+    (76, 8, 1, 110, 128, ()),                         # two
+    (40, 4, 2, 200, 256, ()),                         # four
+    (40, 4, 1, 60, 1024, ((900, 5), (1010, 7))),      # clusters
+])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("page", [16, 4])             # TMA; pages too short for it
+@pytest.mark.parametrize("tree,holes", [(True, False), (False, True), (True, True)])
+def test_tree_attention_eight_rows_at_a_time(ops, B, Hkv, G, most, width_keys, long, D, page, tree, holes):
+    ctx, new, spare = _many_pairs(B + D + page, B, most, G, width_keys, page, long)
+    c = _attn_case(B + page, ctx, new, Hkv, G, D, page, tree, extra_width=spare, empty_rows=holes)
+    if holes:
+        rng = np.random.default_rng(B)
+        at = rng.integers(0, 8, (c["table"].shape[0], 2)) % np.maximum(1, -(-c["ctx"][:, None] // page))
+        c["table"][np.arange(0, B, 3), at[::3, 0]] = -1
+        c["table"][np.arange(0, B, 5), at[::5, 1]] = 10 ** 6
+    _check_attn(ops, c)
+
+
+@pytest.mark.parametrize("mult,shift,fb,av,off", [(255, 3, 13, (94, 5), 16), (255, 0, 12, (255, 0), 12), (64, 6, 15, (88, 6), 16),
+                                                  (0, 5, 13, (88, 5), 16), (90, 6, 1, (88, 5), 16), (90, 6, 30, (88, 32), 29),
+                                                  (255, 2, 7, (88, 5), 16), (64, 6, 14, (255, 0), 16)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("low", [False, True])
+def test_tree_attention_parameters_eight_rows_at_a_time(ops, mult, shift, fb, av, off, D, low):
+    ctx, new, spare = _many_pairs(fb + D, 150, 50, 1, 64, 16)
+    c = _attn_case(fb, ctx, new, 4, 1, D, 16, True, sd=60, extra_width=spare)
+    if low:  # every score far below 0
+        c["q"], c["kc"] = np.abs(c["q"].astype(np.int16)).clip(1, 127).astype(np.int8), -np.abs(
+            c["kc"].astype(np.int16)).clip(1, 127).astype(np.int8)
+    _check_attn(ops, c, mult, shift, fb, av, off)
+
+
+@pytest.mark.parametrize("D,page,G,tree", [(64, 16, 1, True), (128, 16, 1, False), (64, 4, 2, True), (128, 64, 2, True), (64, 64, 1, False)])
+@pytest.mark.parametrize("holes", [False, True])
+def test_tree_attention_more_scores_than_a_warp_keeps(ops, D, page, G, tree, holes):
+    """Requests of 20000 keys and several rows among short ones: their scores do not fit shared memory and are
+    computed again from K in global memory in the second pass."""
+    ctx, new, spare = _many_pairs(D + page, 20, 300, G, 65536, page, ((20000, 8), (19000, 11)))
+    c = _attn_case(D * G + page, ctx, new, 1, G, D, page, tree, extra_width=spare)
+    if holes:
+        c["table"][0, 7], c["table"][0, 200], c["table"][1, 1] = -1, 10 ** 6, -1
+    _check_attn(ops, c, 70, 7)
+
+
 def test_no_wait_ran_out(ops):
     from i_whisper_b200 import _lib
     assert _lib.device_status(clear=True) == 0
