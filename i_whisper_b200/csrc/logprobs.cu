@@ -97,7 +97,7 @@ IW_DEV T block_reduce(T v, F f, T *red) {
 
 // A row cut into 16-byte vectors: `head` elements before the first aligned one,
 // `vecs` vectors, `tail` elements. Vector v belongs to thread v % (threads),
-// head and tail element e to thread e (they are fewer than 16).
+// head and tail elements, fewer than 16 each, to the first `head + tail` threads.
 template <typename T>
 struct Row {
     static constexpr int kPer = 16 / sizeof(T);
@@ -157,7 +157,9 @@ IW_DEV float max_nan(float a, float b) {
 }
 
 template <typename T, bool SUP, int kThreads>
-__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) == 1 ? 6 : 3)) token_logprobs_kernel(LogprobsArgs a) {
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : (sizeof(T) == 1 ? 5 : 3)) token_logprobs_kernel(LogprobsArgs a) {
+    // int8: five blocks' histograms fill an SM's shared memory
+    static_assert(kThreads >= 32, "a thread for every element outside the vectors");
     constexpr bool kBytes = sizeof(T) == 1;
     constexpr int P = Row<T>::kPer, kWarps = kThreads / 32;
     pdl_wait();
