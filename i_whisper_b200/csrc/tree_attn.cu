@@ -606,11 +606,12 @@ __global__ void __launch_bounds__(32 * W, (D == 64 ? 20 : 12) / W)
 // at all where K and V of the request fit the ring.
 // 64 requests with trees of 5 to 32 tokens over 64 to 416 keys, 16 heads of 64:
 // 39 us. 16 requests with trees of 24 to 64 tokens over 1000 to 8191 keys, 32 query
-// and 8 key heads of 128: 295 us, 0.3 of what mma.sync does in 8 bits (1.09 POPS
+// and 8 key heads of 128: 298 us, 0.27 of what mma.sync does in 8 bits (1.09 POPS
 // measured). More warps per SM, with fewer registers each or the query
 // operands in shared memory, measured 296 to 310 us. tcgen05 would multiply
 // faster, but hold the scores in tensor memory, from where the softmax has to
-// fetch them, and it wants 128 rows, which trees on one head do not have.
+// fetch them; not measured. Trees on one head have too few rows for its 128-row
+// tiles, shared key heads (96 to 256 rows in the case above) do not.
 // ---------------------------------------------------------------------------
 constexpr int kManyWarps = 4;
 

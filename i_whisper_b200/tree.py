@@ -207,8 +207,8 @@ class TreeDecoder:
         """Greedy decoding of ``n_tokens`` tokens per utterance, checked in
         drafted trees: ``draft(b, history)`` returns the drafted tokens and
         parents (-1: follows the history) that may continue utterance b. Returns
-        the new tokens, the same whatever is drafted; good drafts take
-        fewer passes (``self.passes``)."""
+        the new tokens (fewer where the text context is full), the same
+        whatever is drafted; good drafts take fewer passes (``self.passes``)."""
         hist = [list(p) for p in prompts]
         if not all(hist):
             raise RuntimeError("greedy needs a prompt of at least one token for every utterance")
